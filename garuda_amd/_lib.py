@@ -111,6 +111,12 @@ SIGNATURES = {
     "gmoe_predictor_set_counts": (i32, [vp, u32p, u64]),
     "gmoe_prefetch_step": (i32, [vp, vp, u32, u32, u32p, u32, u32p, u32, u32p, u32, u32, u32p, u32p, u32p, u32p]),
     "gmoe_kv_create": (i32, [vp, vp, C.POINTER(vp)]),
+    "gmoe_kv_create_q8": (i32, [vp, vp, C.POINTER(vp)]),
+    "gmoe_kv_append": (i32, [vp, u32, vp, u32, f32p, f32p]),
+    "gmoe_kv_append_async": (i32, [vp, u32, vp, u32, vp, vp, vp]),
+    "gmoe_kv_read": (i32, [vp, u32, vp, vp, u32, f32p, f32p]),
+    "gmoe_kv_read_async": (i32, [vp, u32, vp, vp, u32, vp, vp, vp]),
+    "gmoe_kv_truncate": (i32, [vp, vp, vp, u32, vp]),
     "gmoe_kv_destroy": (None, [vp]),
     "gmoe_kv_seq_open": (i32, [vp, u32p]),
     "gmoe_kv_seq_close": (i32, [vp, u32]),

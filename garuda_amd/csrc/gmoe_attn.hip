@@ -1005,6 +1005,35 @@ hipError_t launch_attention(const AttnArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
+hipError_t launch_append(const AttnArgs& a, hipStream_t st) {
+  const uint32_t pairs = a.n_kv * a.hd / 2;
+  hipLaunchKernelGGL(k_rope_append, dim3(a.n, (pairs + 255) / 256), dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+// grid (chunks, n_kv), 256 threads: a chunk's rows of one kv head, keys and values. Pages
+// hold [2][n_kv][bs][hd] f32.
+__global__ void __launch_bounds__(256) k_kv_read(Kv8Pool p, const float* pool, const Kv8Rows* rows, Kv8RowsInline inl,
+                                                 float* k, float* v) {
+  const Kv8Rows r = rows ? rows[blockIdx.x] : inl.r[blockIdx.x];
+  const uint32_t h = blockIdx.y, kvd = p.n_kv * p.hd;
+  const uint32_t page = p.tables[(size_t)r.table * p.ppseq + r.block];
+  const float* src = pool + (size_t)page * 2 * p.bs * kvd + ((size_t)h * p.bs + r.r0) * p.hd;
+  float* dk = k + (size_t)r.i0 * kvd + h * p.hd;
+  float* dv = v + (size_t)r.i0 * kvd + h * p.hd;
+  for (uint32_t x = threadIdx.x; x < r.n * p.hd; x += 256) {
+    const size_t to = (size_t)(x / p.hd) * kvd + x % p.hd;
+    dk[to] = src[x];
+    dv[to] = src[(size_t)p.bs * kvd + x];
+  }
+}
+
+hipError_t launch_kv_read(const Kv8Pool& p, const float* pool, const Kv8Rows* rows, const Kv8RowsInline& inl,
+                          uint32_t nrows, float* k, float* v, hipStream_t st) {
+  hipLaunchKernelGGL(k_kv_read, dim3(nrows, p.n_kv), dim3(256), 0, st, p, pool, rows, inl, k, v);
+  return hipGetLastError();
+}
+
 hipError_t launch_attention_tiled(const AttnArgs& a, const AttnArgs& rest, hipStream_t st) {
   hipLaunchKernelGGL(k_rope_rows, dim3(a.n, 2), dim3(256), 0, st, a);  // every entry's k and v before any attends
   const dim3 grid(a.n_kv, a.ntile, a.nchunk);

@@ -469,6 +469,83 @@ hipError_t launch_attention(const AttnArgs& a, hipStream_t st);
 hipError_t launch_attention_tiled(const AttnArgs& a, const AttnArgs& rest, hipStream_t st);
 constexpr bool attn_tiled_hd(uint32_t hd) { return hd % 32 == 0 && hd <= 128; }
 
+// ---- the KV cache held in 8 bits (gmoe_attn8.hip) ----
+// Positions are held in blocks of 16. A complete block of one (sequence, layer, kv head) is
+// 16 hdp bytes of key codes, then 16 hdp of value codes, each code + 128, hdp being the head
+// width rounded up by kv8_width (the codes past it stand for 0), with an f32 scale for the
+// keys and one for the values. Keys: steps of 64 dims [16 rows][64], a last step of 32 where
+// hdp is no multiple of 64; values: [hdp][16 rows]. The block of a sequence's last position
+// is held in f32 besides (`open`), and by itself while it is incomplete.
+constexpr uint32_t kKv8Block = 16;
+constexpr uint32_t kv8_width(uint32_t hd) { return hd <= 128 ? (hd + 31) / 32 * 32 : (hd + 63) / 64 * 64; }
+struct Kv8Pool {
+  uint8_t* codes;       // [max_pages][n_kv][bs / 16][2][16 hdp]
+  float* scales;        // [max_pages][n_kv][bs / 16][2] (keys, values); NaN: a value that is not finite
+  float* open;          // [max_seqs][n_layers][2][n_kv][16][hd]: the rows of the last position's block
+  uint32_t* tables;     // [max_seqs][n_layers][ppseq]
+  const double* turns;  // [hd / 2]: theta^(-2i/hd) / (2 pi)
+  uint32_t n_kv, hd, hdp, bs, ppseq;
+};
+// One block that a call appends to: every row before r0 was there before the call, row r from
+// r0 on is entry ent[r] (rows below r0 + n). Jobs of one sequence follow each other.
+constexpr uint32_t kKv8Fresh = 1, kKv8Whole = 2, kKv8First = 4;
+struct Kv8Job {
+  uint32_t table;  // index of the sequence's page table, and of its open rows
+  uint32_t block, page;
+  uint32_t flags;  // Fresh: the block opens the page; Whole: the call completes it; First: of its sequence
+  uint32_t r0, n;
+  uint32_t last;   // the job of the sequence's last block
+  uint32_t pad;
+  uint32_t ent[kKv8Block];
+};
+// Consecutive entries of one sequence, from entry i0 and position pos0 on; job: of pos0's block.
+struct Kv8Run {
+  uint32_t i0, n, pos0, job, table;
+};
+// Rows r0 .. r0 + n - 1 of one block (a cache in f32: of the sequence's page `block`), n <= 16:
+// output rows i0 .. i0 + n - 1 of a read. whole: from the codes, otherwise from the open rows.
+struct Kv8Rows {
+  uint32_t table, block, i0, r0, n, whole;
+};
+constexpr uint32_t kKv8Inline = 64;  // entries, or blocks of a read, carried in the kernel arguments
+struct Kv8Args {
+  Kv8Pool p;
+  const AttnEntry* ent;  // [n] in device memory; null: a step's n <= kKv8Inline entries ride beside (Kv8Inline)
+  uint32_t n, n_heads, window;
+  float scale;
+  const float *q, *k, *v;
+  uint32_t q_stride, kv_stride;  // floats between rows of q, and of k and v
+  uint32_t nsl;                  // > 1: q, k and v are sums of nsl slices sl_stride floats apart
+  uint64_t sl_stride;
+  float* ctx;
+  const Kv8Job* hjob;  // [njob] in pinned host memory, and the runs; k8_append copies them to
+  const Kv8Run* hrun;  //   run for the launches after it
+  Kv8Run* run;
+  float* own;          // [njob][2][n_kv][16][hd]: the jobs' f32 rows, keys rotated; null: not wanted
+  uint32_t njob, nrun;
+};
+struct Kv8Inline {
+  AttnEntry e[kKv8Inline];
+};
+// Attention of one token of each of n different sequences, appended on the way.
+hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st);
+// Appends the call's jobs; then attention of its runs, where a.ctx is given.
+hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st);
+// Rows of blocks to k and v [n][n_kv * hd]: nrows of them, in `inl` when they are at most kKv8Inline,
+// else in `rows` (memory that the device reads).
+struct Kv8RowsInline {
+  Kv8Rows r[kKv8Inline];
+};
+hipError_t launch_kv8_read(const Kv8Pool& p, const Kv8Rows* rows, const Kv8RowsInline& inl, uint32_t nrows, float* k,
+                           float* v, hipStream_t st);
+// Rows of complete blocks to their sequences' open rows (nrows <= kKv8Inline).
+hipError_t launch_kv8_reopen(const Kv8Pool& p, const Kv8RowsInline& inl, uint32_t nrows, hipStream_t st);
+// Keys and values appended to a cache in f32 (k_rope_append without queries).
+hipError_t launch_append(const AttnArgs& a, hipStream_t st);
+// launch_kv8_read of a cache in f32, whose pages are `pool`.
+hipError_t launch_kv_read(const Kv8Pool& p, const float* pool, const Kv8Rows* rows, const Kv8RowsInline& inl,
+                          uint32_t nrows, float* k, float* v, hipStream_t st);
+
 // Decode-step glue (gmoe_glue.hip): embedding rows, residual add + RMSNorm * weight,
 // greedy token. A decode step carries its tokens in the kernel arguments.
 constexpr uint32_t kModelMaxBatch = 64;

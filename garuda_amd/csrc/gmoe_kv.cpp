@@ -6,7 +6,8 @@
 // blocks are pages of one device pool shared by every sequence and layer; the host keeps
 // each (sequence, layer)'s length and page list, and the device keeps its page table,
 // which the append kernel extends when a token opens a page. attend_one
-// (llama/mod.rs:766-821) runs as one to five launches (gmoe_attn.hip).
+// (llama/mod.rs:766-821) runs as one to five launches (gmoe_attn.hip). A cache may hold its
+// complete blocks of 16 positions in 8 bits (gmoe_kv_create_q8, gmoe_attn8.hip).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -16,6 +17,8 @@
 #include <cstring>
 #include <memory>
 #include <mutex>
+#include <new>
+#include <stdexcept>
 #include <vector>
 
 #include "../../include/garuda_moe.h"
@@ -41,6 +44,18 @@ gmoe_status kfail(gmoe_status s, const char* fmt, ...) {
   return s;
 }
 
+// The body of a C entry whose host planning allocates: no exception leaves it.
+template <class F>
+gmoe_status guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return kfail(GMOE_ERR_DEVICE, "no host memory for the call's plan");
+  } catch (const std::length_error&) {
+    return kfail(GMOE_ERR_DEVICE, "no host memory for the call's plan");
+  }
+}
+
 #define KV_TRY(expr)                                                                       \
   do {                                                                                     \
     hipError_t e_ = (expr);                                                                \
@@ -55,6 +70,7 @@ struct Seq {
   bool open = false;
   std::vector<uint32_t> len;                 // [layer]
   std::vector<std::vector<uint32_t>> pages;  // [layer] page ids in position order
+  std::vector<uint32_t> open_block;          // [layer] 8 bits: the block whose rows the open rows are
 };
 
 }  // namespace
@@ -64,7 +80,9 @@ struct gmoe_kv {
   gmoe_kv_desc d{};
   uint32_t kvd = 0, ppseq = 0;
   uint64_t page_floats = 0;
-  float* pool = nullptr;      // [max_pages][2][block_size][kvd]
+  float* pool = nullptr;      // [max_pages][2][block_size][kvd]; null in 8 bits
+  bool q8 = false;            // complete blocks held in 8 bits
+  Kv8Pool p8{};               // (with its tables and widths; a cache in f32 has only those)
   uint32_t* tables = nullptr; // [max_seqs][n_layers][ppseq]
   std::vector<uint32_t> free_pages;
   std::vector<Seq> seqs;
@@ -76,12 +94,18 @@ struct gmoe_kv {
   size_t pin_half = 0, pin_at = 0;
   hipEvent_t pin_ev[2]{};
   int pin_cur = 0;
+  float* saved = nullptr;      // 8 bits: a sequence's open rows, kept while a prompt runs (kv_snapshot)
   uint32_t fail_reserves = 0;  // test hook: reservations still to refuse (gmoe_kv_fail_reserves)
   std::mutex mu;
 
   ~gmoe_kv() {
     if (pool) hipFree(pool);
     if (tables) hipFree(tables);
+    if (p8.codes) hipFree(p8.codes);
+    if (p8.scales) hipFree(p8.scales);
+    if (p8.open) hipFree(p8.open);
+    if (p8.turns) hipFree(const_cast<double*>(p8.turns));
+    if (saved) hipFree(saved);
     if (scratch) hipFree(scratch);
     if (pin) hipHostFree(pin);
     for (auto& e : pin_ev)
@@ -178,6 +202,7 @@ void commit(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, AttnE
     }
     ent[i].page = S.pages[layer][ent[i].pos / D.block_size];
     S.len[layer] = ent[i].pos + 1;
+    S.open_block[layer] = ent[i].pos / kKv8Block;
   }
 }
 
@@ -279,10 +304,243 @@ AttnArgs args(const gmoe_kv* kv, uint32_t n, uint32_t nchunk, const AttnLayout& 
   return a;
 }
 
+// The calls that read their plan's pinned memory, or that advance the host's lengths, cannot
+// be replayed: a graph would run them again on the memory of later calls.
+gmoe_status refuse_capture(hipStream_t st) {
+  hipStreamCaptureStatus c = hipStreamCaptureStatusNone;
+  KV_TRY(hipStreamIsCapturing(st, &c));
+  if (c != hipStreamCaptureStatusNone)
+    return kfail(GMOE_ERR_INFERENCE, "a call that plans on the host cannot be captured into a graph");
+  return GMOE_OK;
+}
+
+Kv8Args args8(const gmoe_kv* kv, uint32_t n, const float* q, const float* k, const float* v, float* out,
+              uint32_t q_stride, uint32_t kv_stride) {
+  const gmoe_kv_desc& D = kv->d;
+  Kv8Args a{};
+  a.p = kv->p8;
+  a.n = n;
+  a.n_heads = D.n_heads;
+  a.window = D.sliding_window;
+  a.scale = 1.0f / std::sqrt((float)D.head_dim);
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.ctx = out;
+  a.q_stride = q_stride ? q_stride : D.n_heads * D.head_dim;
+  a.kv_stride = kv_stride ? kv_stride : kv->kvd;
+  return a;
+}
+
+// The blocks that a planned call appends to, those of one sequence in position order, and its
+// runs (pages: job_pages, after the commit).
+void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEntry* ent, std::vector<Kv8Job>& jobs,
+               std::vector<Kv8Run>& runs) {
+  struct Of {
+    uint32_t count = 0, pos0 = 0, job = 0;
+  };
+  std::vector<Of> of(kv->seqs.size());
+  for (uint32_t i = 0; i < n; i++) {
+    Of& o = of[seqs[i]];
+    if (!o.count++) o.pos0 = ent[i].pos;
+  }
+  for (uint32_t i = 0; i < n; i++) {
+    Of& o = of[seqs[i]];
+    const uint32_t block = ent[i].pos / kKv8Block, row = ent[i].pos % kKv8Block;
+    const uint32_t table = (uint32_t)((ent[i].pages - kv->tables) / kv->ppseq);
+    if (ent[i].pos == o.pos0) {
+      o.job = (uint32_t)jobs.size();
+      const uint32_t nb = (o.pos0 % kKv8Block + o.count + kKv8Block - 1) / kKv8Block;
+      for (uint32_t b = 0; b < nb; b++) {
+        Kv8Job j{};
+        j.table = table;
+        j.block = block + b;
+        j.r0 = b ? 0 : row;
+        j.n = std::min(kKv8Block - j.r0, o.pos0 + o.count - (j.block * kKv8Block + j.r0));
+        j.flags = (b ? 0 : kKv8First) | (j.r0 + j.n == kKv8Block ? kKv8Whole : 0);
+        j.last = o.job + nb - 1;
+        jobs.push_back(j);
+      }
+    }
+    jobs[o.job + block - o.pos0 / kKv8Block].ent[row] = i;
+    if (i && ent[i - 1].pages == ent[i].pages) runs.back().n++;
+    else runs.push_back(Kv8Run{i, 1, ent[i].pos, o.job + block - o.pos0 / kKv8Block, table});
+  }
+}
+
+void job_pages(std::vector<Kv8Job>& jobs, const AttnEntry* ent) {
+  for (Kv8Job& j : jobs) {
+    const AttnEntry& e = ent[j.ent[j.r0]];
+    j.page = e.page;
+    if (e.fresh) j.flags |= kKv8Fresh;  // a page opens with a block
+  }
+}
+
+// attend() for a cache in 8 bits; with `out` null the tokens are only appended.
+gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* q, const float* k,
+                    const float* v, float* out, hipStream_t st, uint32_t q_stride, uint32_t kv_stride) {
+  if (gmoe_status s = refuse_capture(st)) return s;
+  std::vector<AttnEntry> ent(n ? n : 1);
+  uint32_t maxspan;
+  bool distinct;
+  if (gmoe_status s = plan(kv, layer, seqs, n, ent.data(), &maxspan, &distinct)) return s;
+  Kv8Args a = args8(kv, n, q, k, v, out, q_stride, kv_stride);
+  uint8_t* pin = nullptr;
+  if (out && distinct) {
+    Kv8Inline inl{};
+    const size_t eb = n * sizeof(AttnEntry);
+    if (n > kKv8Inline) {
+      if (gmoe_status s = grow_scratch(kv, eb)) return s;
+      if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
+    }
+    commit(kv, layer, seqs, n, ent.data());
+    if (pin) {
+      memcpy(pin, ent.data(), eb);
+      KV_TRY(hipMemcpyAsync(kv->scratch, pin, eb, hipMemcpyHostToDevice, st));
+      a.ent = reinterpret_cast<const AttnEntry*>(kv->scratch);
+    } else {
+      std::copy(ent.begin(), ent.begin() + n, inl.e);
+    }
+    KV_TRY(launch_kv8_step(a, inl, st));
+    return GMOE_OK;
+  }
+  std::vector<Kv8Job> jobs;
+  std::vector<Kv8Run> runs;
+  find_jobs(kv, seqs, n, ent.data(), jobs, runs);
+  const size_t jb = jobs.size() * sizeof(Kv8Job), rb = runs.size() * sizeof(Kv8Run), o_own = (rb + 255) & ~(size_t)255;
+  if (out)
+    if (gmoe_status s = grow_scratch(kv, o_own + jobs.size() * 2 * kKv8Block * kv->kvd * 4)) return s;
+  if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
+  commit(kv, layer, seqs, n, ent.data());
+  job_pages(jobs, ent.data());
+  memcpy(pin, jobs.data(), jb);
+  memcpy(pin + jb, runs.data(), rb);
+  a.hjob = reinterpret_cast<const Kv8Job*>(pin);
+  a.hrun = reinterpret_cast<const Kv8Run*>(pin + jb);
+  a.njob = (uint32_t)jobs.size();
+  a.nrun = (uint32_t)runs.size();
+  if (out) {
+    a.run = reinterpret_cast<Kv8Run*>(kv->scratch);
+    a.own = reinterpret_cast<float*>(kv->scratch + o_own);
+  }
+  KV_TRY(launch_kv8_call(a, st));
+  return GMOE_OK;
+}
+
+// The call's keys and values appended.
+gmoe_status append(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* k, const float* v,
+                   hipStream_t st) {
+  if (kv->q8) return attend8(kv, layer, seqs, n, nullptr, k, v, nullptr, st, 0, 0);
+  if (gmoe_status s = refuse_capture(st)) return s;
+  std::vector<AttnEntry> ent(n ? n : 1);
+  uint32_t maxspan;
+  if (gmoe_status s = plan(kv, layer, seqs, n, ent.data(), &maxspan)) return s;
+  AttnArgs a = args(kv, n, 0, AttnLayout{}, nullptr, k, v, nullptr, 0, 0);
+  a.n_heads = 0;  // no queries
+  uint8_t* pin = nullptr;
+  if (n > kAttnInline)
+    if (gmoe_status s = take_pinned(kv, n * sizeof(AttnEntry), st, &pin)) return s;
+  commit(kv, layer, seqs, n, ent.data());
+  if (pin) {
+    memcpy(pin, ent.data(), n * sizeof(AttnEntry));
+    a.ent = reinterpret_cast<const AttnEntry*>(pin);
+  } else {
+    std::copy(ent.begin(), ent.begin() + n, a.inl);
+  }
+  KV_TRY(launch_append(a, st));
+  return GMOE_OK;
+}
+
+// The rows at positions pos[i] of seqs[i], in pieces of a block (in f32: of a page).
+gmoe_status read_rows(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const uint32_t* pos, uint32_t n, float* k,
+                      float* v, hipStream_t st) {
+  const gmoe_kv_desc& D = kv->d;
+  if (layer >= D.n_layers) return kfail(GMOE_ERR_INFERENCE, "layer %u of %u", layer, D.n_layers);
+  if (n == 0 || !seqs || !pos) return kfail(GMOE_ERR_INFERENCE, "empty read");
+  if (gmoe_status s = refuse_capture(st)) return s;
+  std::vector<Kv8Rows> rows;
+  const uint32_t per = kv->q8 ? kKv8Block : D.block_size;
+  for (uint32_t i = 0; i < n; i++) {
+    const uint32_t s = seqs[i];
+    if (s >= kv->seqs.size() || !kv->seqs[s].open) return kfail(GMOE_ERR_INFERENCE, "sequence %u is not open", s);
+    const uint32_t len = kv->seqs[s].len[layer], b = pos[i] / per, r = pos[i] % per;
+    if (pos[i] >= len) return kfail(GMOE_ERR_INFERENCE, "position %u of a sequence of %u", pos[i], len);
+    const uint32_t table = s * D.n_layers + layer;
+    if (!rows.empty()) {
+      Kv8Rows& l = rows.back();
+      if (l.table == table && l.block == b && l.r0 + l.n == r && l.n < kKv8Block) {
+        l.n++;
+        continue;
+      }
+    }
+    rows.push_back(Kv8Rows{table, b, i, r, 1, kv->q8 && (uint64_t)(b + 1) * kKv8Block <= len});
+  }
+  Kv8RowsInline inl{};
+  uint8_t* pin = nullptr;
+  const size_t bytes = rows.size() * sizeof(Kv8Rows);
+  if (rows.size() > kKv8Inline) {
+    if (gmoe_status s = take_pinned(kv, bytes, st, &pin)) return s;
+    memcpy(pin, rows.data(), bytes);
+  } else {
+    std::copy(rows.begin(), rows.end(), inl.r);
+  }
+  const Kv8Rows* list = reinterpret_cast<const Kv8Rows*>(pin);
+  if (kv->q8) KV_TRY(launch_kv8_read(kv->p8, list, inl, (uint32_t)rows.size(), k, v, st));
+  else KV_TRY(launch_kv_read(kv->p8, kv->pool, list, inl, (uint32_t)rows.size(), k, v, st));
+  return GMOE_OK;
+}
+
+// Sequence s goes back to at most len positions in `layer`: pages past them are free again.
+// Returns whether its open rows have to be made again from codes.
+bool take_back(gmoe_kv* kv, uint32_t s, uint32_t layer, uint32_t len, Kv8Rows* rows) {
+  Seq& S = kv->seqs[s];
+  if (S.len[layer] <= len) return false;
+  S.len[layer] = len;
+  const uint32_t keep = (uint32_t)(((uint64_t)len + kv->d.block_size - 1) / kv->d.block_size);
+  while (S.pages[layer].size() > keep) {
+    kv->free_pages.push_back(S.pages[layer].back());
+    S.pages[layer].pop_back();
+  }
+  const uint32_t b = len / kKv8Block;
+  if (!kv->q8 || len % kKv8Block == 0 || S.open_block[layer] == b) return false;
+  S.open_block[layer] = b;
+  *rows = Kv8Rows{s * kv->d.n_layers + layer, b, 0, 0, len % kKv8Block, 1};
+  return true;
+}
+
+gmoe_status truncate(gmoe_kv* kv, const uint32_t* seqs, const uint32_t* lens, uint32_t n, hipStream_t st) {
+  if (n == 0 || !seqs || !lens) return kfail(GMOE_ERR_INFERENCE, "no sequences or lengths");
+  if (gmoe_status s = refuse_capture(st)) return s;
+  for (uint32_t i = 0; i < n; i++)
+    if (seqs[i] >= kv->seqs.size() || !kv->seqs[seqs[i]].open)
+      return kfail(GMOE_ERR_INFERENCE, "sequence %u is not open", seqs[i]);
+  Kv8RowsInline inl{};
+  uint32_t m = 0;
+  for (uint32_t i = 0; i < n; i++) {
+    // named before: its earlier rows may be waiting in inl
+    if (m)
+      for (uint32_t j = 0; j < i; j++)
+        if (seqs[j] == seqs[i]) {
+          KV_TRY(launch_kv8_reopen(kv->p8, inl, m, st));
+          m = 0;
+          break;
+        }
+    for (uint32_t l = 0; l < kv->d.n_layers; l++) {
+      if (!take_back(kv, seqs[i], l, lens[i], &inl.r[m])) continue;
+      if (++m < kKv8Inline) continue;
+      KV_TRY(launch_kv8_reopen(kv->p8, inl, m, st));
+      m = 0;
+    }
+  }
+  if (m) KV_TRY(launch_kv8_reopen(kv->p8, inl, m, st));
+  return GMOE_OK;
+}
+
 // Plans the call's entries and commits them (lengths advance and pages are taken only when
 // the whole call fits), then queues the launches.
 gmoe_status attend(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* q, const float* k,
                    const float* v, float* out, hipStream_t st, uint32_t q_stride = 0, uint32_t kv_stride = 0) {
+  if (kv->q8) return guarded([&] { return attend8(kv, layer, seqs, n, q, k, v, out, st, q_stride, kv_stride); });
   std::vector<AttnEntry> ent(n ? n : 1);
   uint32_t maxspan;
   bool distinct;
@@ -443,29 +701,49 @@ void kv_commit_step(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, AttnEntry* en
   for (uint32_t l = 0; l < kv->d.n_layers; l++) commit(kv, l, seqs, n, ents + (size_t)l * stride);
 }
 
+static size_t open_bytes(const gmoe_kv* kv) { return (size_t)kv->d.n_layers * 2 * kKv8Block * kv->kvd * 4; }  // a sequence's open rows, every layer's
+
 // The step's sequences as they stand (every layer's length and page count), and their
 // return to it: pages taken since go back to the free list, lengths go back. A step that
 // fails after committing positions restores them, so a refused step leaves every sequence
 // where it was.
-void kv_snapshot(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, std::vector<uint32_t>& snap) {
+gmoe_status kv_snapshot(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, std::vector<uint32_t>& snap, bool prompt) {
   std::lock_guard<std::mutex> g(kv->mu);
   snap.clear();
+  // a prompt's rows move a sequence's open rows on to later blocks (a decode step's, at most
+  // to one that it begins): copied before, so that a failed prompt can put them back
+  if (kv->q8 && prompt) {
+    const size_t bytes = open_bytes(kv);
+    KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+    if (!kv->saved) KV_TRY(hipMalloc(&kv->saved, bytes));
+    KV_TRY(hipMemcpyAsync(kv->saved, kv->p8.open + seqs[0] * (bytes / 4), bytes, hipMemcpyDeviceToDevice,
+                          ctx_stream(kv->ctx)));
+  }
   for (uint32_t i = 0; i < n; i++) {
     const Seq& S = kv->seqs[seqs[i]];
     for (uint32_t l = 0; l < kv->d.n_layers; l++) {
       snap.push_back(S.len[l]);
       snap.push_back((uint32_t)S.pages[l].size());
+      snap.push_back(S.open_block[l]);
     }
   }
+  return GMOE_OK;
 }
 
-void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector<uint32_t>& snap) {
+void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector<uint32_t>& snap, bool prompt) {
   std::lock_guard<std::mutex> g(kv->mu);
+  if (kv->q8 && prompt) {
+    const size_t bytes = open_bytes(kv);
+    (void)hipMemcpyAsync(kv->p8.open + seqs[0] * (bytes / 4), kv->saved, bytes, hipMemcpyDeviceToDevice,
+                         ctx_stream(kv->ctx));
+  }
   size_t at = 0;
-  for (uint32_t i = 0; i < n && at + 2 * kv->d.n_layers <= snap.size(); i++) {
+  for (uint32_t i = 0; i < n && at + 3 * kv->d.n_layers <= snap.size(); i++) {
     Seq& S = kv->seqs[seqs[i]];
-    for (uint32_t l = 0; l < kv->d.n_layers; l++, at += 2) {
+    for (uint32_t l = 0; l < kv->d.n_layers; l++, at += 3) {
       S.len[l] = snap[at];
+      // a step leaves the open rows at its token's block: earlier ones come back from codes
+      if (prompt) S.open_block[l] = snap[at + 2];
       while (S.pages[l].size() > snap[at + 1]) {
         kv->free_pages.push_back(S.pages[l].back());
         S.pages[l].pop_back();
@@ -500,6 +778,15 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
                           const float* k, const float* v, uint32_t q_stride, uint32_t kv_stride, float* out,
                           hipStream_t st, uint32_t nsl, uint64_t sl_stride) {
   std::lock_guard<std::mutex> g(kv->mu);
+  if (kv->q8) {
+    if (nsl > kMaxKsg) return kfail(GMOE_ERR_INFERENCE, "%u K slices exceed %u", nsl, kMaxKsg);
+    Kv8Args a = args8(kv, n, q, k, v, out, q_stride, kv_stride);
+    a.ent = d_ent;
+    a.nsl = nsl;
+    a.sl_stride = sl_stride;
+    KV_TRY(launch_kv8_step(a, Kv8Inline{}, st));
+    return GMOE_OK;
+  }
   const AttnLayout l = layout(kv, n, nchunk);
   if (l.total > kv->scratch_bytes) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
   if (nsl > kMaxKsg) return kfail(GMOE_ERR_INFERENCE, "%u K slices exceed %u", nsl, kMaxKsg);
@@ -516,7 +803,7 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
 
 extern "C" {
 
-gmoe_status gmoe_kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out) {
+static gmoe_status kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, bool q8, gmoe_kv** out) {
   if (!ctx || !desc || !out) return kfail(GMOE_ERR_INFERENCE, "null context, descriptor or output");
   *out = nullptr;
   const gmoe_kv_desc& D = *desc;
@@ -529,6 +816,9 @@ gmoe_status gmoe_kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** ou
   if (D.head_dim % 4 || D.head_dim > kAttnMaxHd)
     return kfail(GMOE_ERR_MODEL, "head_dim %u must be a multiple of 4 and at most %u", D.head_dim, kAttnMaxHd);
   if (!(D.rope_theta > 0.0f)) return kfail(GMOE_ERR_CONFIG, "rope_theta must be positive");
+  if (q8 && D.block_size % kKv8Block)
+    return kfail(GMOE_ERR_MODEL, "block_size %u must be a multiple of %u, the positions that share a scale", D.block_size,
+                 kKv8Block);
   std::unique_ptr<gmoe_kv> kv(new gmoe_kv);
   kv->ctx = ctx;
   kv->d = D;
@@ -536,14 +826,42 @@ gmoe_status gmoe_kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** ou
   kv->ppseq = (D.max_positions + D.block_size - 1) / D.block_size;
   kv->page_floats = 2ull * D.block_size * kv->kvd;
   KV_TRY(hipSetDevice(ctx_device(ctx)));
-  KV_TRY(hipMalloc(&kv->pool, D.max_pages * kv->page_floats * 4));
   KV_TRY(hipMalloc(&kv->tables, (size_t)D.max_seqs * D.n_layers * kv->ppseq * 4));
+  kv->q8 = q8;
+  Kv8Pool& P = kv->p8;
+  P.tables = kv->tables;
+  P.n_kv = D.n_kv_heads;
+  P.hd = D.head_dim;
+  P.hdp = kv8_width(D.head_dim);
+  P.bs = D.block_size;
+  P.ppseq = kv->ppseq;
+  if (q8) {
+    const size_t units = D.max_pages * (D.block_size / kKv8Block) * D.n_kv_heads;
+    KV_TRY(hipMalloc(&P.codes, units * 2 * kKv8Block * P.hdp));
+    KV_TRY(hipMalloc(&P.scales, units * 2 * sizeof(float)));
+    KV_TRY(hipMalloc(&P.open, (size_t)D.max_seqs * D.n_layers * 2 * kKv8Block * kv->kvd * 4));
+    std::vector<double> turns(D.head_dim / 2);
+    for (uint32_t i = 0; i < turns.size(); i++)
+      turns[i] = std::pow((double)D.rope_theta, -(2.0 * i) / D.head_dim) / 6.283185307179586476925286766559;
+    KV_TRY(hipMalloc((void**)&P.turns, turns.size() * sizeof(double)));
+    KV_TRY(hipMemcpy(const_cast<double*>(P.turns), turns.data(), turns.size() * sizeof(double), hipMemcpyHostToDevice));
+  } else {
+    KV_TRY(hipMalloc(&kv->pool, D.max_pages * kv->page_floats * 4));
+  }
   for (auto& e : kv->pin_ev) KV_TRY(hipEventCreateWithFlags(&e, hipEventDisableTiming));
   kv->free_pages.resize(D.max_pages);
   for (uint64_t i = 0; i < D.max_pages; i++) kv->free_pages[i] = (uint32_t)(D.max_pages - 1 - i);  // pops 0 first
   kv->seqs.resize(D.max_seqs);
   *out = kv.release();
   return GMOE_OK;
+}
+
+gmoe_status gmoe_kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out) {
+  return kv_create(ctx, desc, false, out);
+}
+
+gmoe_status gmoe_kv_create_q8(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out) {
+  return kv_create(ctx, desc, true, out);
 }
 
 void gmoe_kv_destroy(gmoe_kv* kv) {
@@ -562,6 +880,7 @@ gmoe_status gmoe_kv_seq_open(gmoe_kv* kv, uint32_t* seq) {
       S.open = true;
       S.len.assign(kv->d.n_layers, 0);
       S.pages.assign(kv->d.n_layers, {});
+      S.open_block.assign(kv->d.n_layers, 0);
       *seq = s;
       return GMOE_OK;
     }
@@ -635,6 +954,75 @@ gmoe_status gmoe_attention_async(gmoe_kv* kv, uint32_t layer, const uint32_t* se
   std::lock_guard<std::mutex> g(kv->mu);
   KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
   return attend(kv, layer, seqs, n, d_q, d_k, d_v, d_context, stream ? (hipStream_t)stream : ctx_stream(kv->ctx));
+}
+
+gmoe_status gmoe_kv_append(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* k,
+                           const float* v) {
+  if (!kv || !k || !v) return kfail(GMOE_ERR_INFERENCE, "null cache, keys or values");
+  if (n == 0) return kfail(GMOE_ERR_INFERENCE, "empty append");
+  std::lock_guard<std::mutex> g(kv->mu);
+  KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+  const size_t kb = (size_t)n * kv->kvd * 4;
+  float* buf = nullptr;
+  KV_TRY(hipMalloc(&buf, 2 * kb));
+  hipStream_t st = ctx_stream(kv->ctx);
+  hipError_t e = hipMemcpyAsync(buf, k, kb, hipMemcpyHostToDevice, st);
+  if (e == hipSuccess) e = hipMemcpyAsync(buf + kb / 4, v, kb, hipMemcpyHostToDevice, st);
+  gmoe_status s = e == hipSuccess ? guarded([&] { return append(kv, layer, seqs, n, buf, buf + kb / 4, st); })
+                                  : kfail(GMOE_ERR_DEVICE, "append inputs: %s", hipGetErrorString(e));
+  e = hipStreamSynchronize(st);
+  hipFree(buf);
+  if (s == GMOE_OK && e != hipSuccess) s = kfail(GMOE_ERR_DEVICE, "append: %s", hipGetErrorString(e));
+  return s;
+}
+
+gmoe_status gmoe_kv_append_async(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* d_k,
+                                 const float* d_v, void* stream) {
+  if (!kv || !d_k || !d_v) return kfail(GMOE_ERR_INFERENCE, "null cache, keys or values");
+  if (n == 0) return kfail(GMOE_ERR_INFERENCE, "empty append");
+  std::lock_guard<std::mutex> g(kv->mu);
+  KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+  const hipStream_t st = stream ? (hipStream_t)stream : ctx_stream(kv->ctx);
+  return guarded([&] { return append(kv, layer, seqs, n, d_k, d_v, st); });
+}
+
+gmoe_status gmoe_kv_read(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const uint32_t* pos, uint32_t n, float* k,
+                         float* v) {
+  if (!kv || !k || !v) return kfail(GMOE_ERR_INFERENCE, "null cache or outputs");
+  if (n == 0) return kfail(GMOE_ERR_INFERENCE, "empty read");
+  std::lock_guard<std::mutex> g(kv->mu);
+  KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+  const size_t kb = (size_t)n * kv->kvd * 4;
+  float* buf = nullptr;
+  KV_TRY(hipMalloc(&buf, 2 * kb));
+  hipStream_t st = ctx_stream(kv->ctx);
+  gmoe_status s = guarded([&] { return read_rows(kv, layer, seqs, pos, n, buf, buf + kb / 4, st); });
+  if (s == GMOE_OK) {
+    hipError_t e = hipMemcpyAsync(k, buf, kb, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipMemcpyAsync(v, buf + kb / 4, kb, hipMemcpyDeviceToHost, st);
+    if (e == hipSuccess) e = hipStreamSynchronize(st);
+    if (e != hipSuccess) s = kfail(GMOE_ERR_DEVICE, "read: %s", hipGetErrorString(e));
+  }
+  hipStreamSynchronize(st);
+  hipFree(buf);
+  return s;
+}
+
+gmoe_status gmoe_kv_read_async(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const uint32_t* pos, uint32_t n,
+                               float* d_k, float* d_v, void* stream) {
+  if (!kv || !d_k || !d_v) return kfail(GMOE_ERR_INFERENCE, "null cache or outputs");
+  std::lock_guard<std::mutex> g(kv->mu);
+  KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+  const hipStream_t st = stream ? (hipStream_t)stream : ctx_stream(kv->ctx);
+  return guarded([&] { return read_rows(kv, layer, seqs, pos, n, d_k, d_v, st); });
+}
+
+gmoe_status gmoe_kv_truncate(gmoe_kv* kv, const uint32_t* seqs, const uint32_t* lens, uint32_t n, void* stream) {
+  if (!kv) return kfail(GMOE_ERR_INFERENCE, "null cache");
+  std::lock_guard<std::mutex> g(kv->mu);
+  KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
+  const hipStream_t st = stream ? (hipStream_t)stream : ctx_stream(kv->ctx);
+  return guarded([&] { return truncate(kv, seqs, lens, n, st); });
 }
 
 }  // extern "C"

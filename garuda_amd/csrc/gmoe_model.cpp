@@ -35,8 +35,8 @@ const void* kv_scratch_id(gmoe_kv* kv);
 gmoe_status kv_plan_step(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, AttnEntry* ents, size_t stride,
                          uint32_t* maxspan);
 void kv_commit_step(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, AttnEntry* ents, size_t stride);
-void kv_snapshot(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, std::vector<uint32_t>& snap);
-void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector<uint32_t>& snap);
+gmoe_status kv_snapshot(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, std::vector<uint32_t>& snap, bool prompt = false);
+void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector<uint32_t>& snap, bool prompt = false);
 gmoe_status ctx_pin_layers(gmoe_ctx* c, const uint32_t* layers, uint32_t n);
 void ctx_unpin_layers(gmoe_ctx* c, const uint32_t* layers, uint32_t n);
 bool dense_tiled(gmoe_ctx* c, uint32_t id, const uint8_t** tiled, uint32_t* qtype);
@@ -533,7 +533,7 @@ static gmoe_status model_decode(gmoe_model* m, uint32_t n, const uint32_t* seqs,
   // device work has finished
   S_TRY(ctx_pin_layers(m->ctx, m->moe.data(), m->n_layers));
   std::vector<uint32_t> snap;
-  kv_snapshot(m->kv, seqs, n, snap);
+  (void)kv_snapshot(m->kv, seqs, n, snap);
   bool capture = false;
   uint32_t cap_chunks = 0;
   const gmoe_status s = decode_body(m, n, seqs, tk, next, logits, trace, &capture, &cap_chunks);
@@ -645,13 +645,13 @@ extern "C" gmoe_status gmoe_model_prefill(gmoe_model* m, uint32_t seq, uint32_t 
       return mfail(GMOE_ERR_INVALID_TOKEN, "token %u is outside the %u-entry vocabulary", tokens[i], m->vocab);
     }
   S_TRY(kv_check_prefill(m->kv, seq, n));
-  S_TRY(ctx_pin_layers(m->ctx, m->moe.data(), m->n_layers));
   std::vector<uint32_t> snap;
-  kv_snapshot(m->kv, &seq, 1, snap);
+  S_TRY(kv_snapshot(m->kv, &seq, 1, snap, true));
+  S_TRY(ctx_pin_layers(m->ctx, m->moe.data(), m->n_layers));
   const gmoe_status s = prefill_body(m, seq, n, tokens, n_last, next, logits);
   if (s != GMOE_OK) {
     (void)hipStreamSynchronize(ctx_stream(m->ctx));
-    kv_restore(m->kv, &seq, 1, snap);
+    kv_restore(m->kv, &seq, 1, snap, true);
   }
   ctx_unpin_layers(m->ctx, m->moe.data(), m->n_layers);
   return s;

@@ -417,6 +417,56 @@ gmoe_status gmoe_attention(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, ui
 gmoe_status gmoe_attention_async(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* d_q,
                                  const float* d_k, const float* d_v, float* d_context, void* stream);
 
+/* A cache as gmoe_kv_create's that holds complete blocks of 16 positions in 8 bits (no
+ * counterpart in the reference, whose cache is f32): about a quarter of the bytes, which
+ * bound the attention of decode steps. Every call on a cache takes either kind.
+ *
+ * Of one sequence, layer and kv head, a block of 16 positions' keys (values) x is held as
+ * integers rint(x * 127 / m), m the largest |x| of the block, and one f32 scale m / 127, and
+ * stands for their product; it is held so from the call on that appends its last position.
+ * The block that a sequence's last position is in is held in f32 besides. A token attends to
+ * the positions of its own block as they were given (keys rotated), and to earlier blocks as
+ * held in 8 bits, so its context does not depend on how the sequence was cut into calls
+ * (but for the rounding of the sums). The rotation's angle is formed in 64 bits and the
+ * rotated pair rounded once to f32; gmoe_kv_create's caches form both in f32, as the
+ * reference does.
+ *
+ * Products and weights keep f32's precision: a query, and a position's softmax weight, is
+ * held as the sum of two fp16 values, to about 2^-22 of the head's largest query element
+ * and of the weight (weights times the value scale that are below 2^-24 of the largest
+ * lose bits, to 2^-39 of it). A block with a NaN or an infinity stands for NaN throughout;
+ * scores that are NaN or +inf, or none above -inf, give uniform weights as in f32.
+ *
+ * block_size must be a multiple of 16. Calls that take a stream plan positions and pages on
+ * the host as they are made, so they are refused while the stream is being captured. */
+gmoe_status gmoe_kv_create_q8(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out);
+/* n tokens' keys and values appended to layer `layer` without attention, entries, positions
+ * and refusals as in gmoe_attention: k and v [n x kv_dim], not yet rotated. A later call
+ * attends to them as if gmoe_attention had appended them (in f32, to the same bits). For a
+ * prompt whose contexts are not wanted, or a prefix whose projections are at hand.
+ * Synchronous; host pointers. */
+gmoe_status gmoe_kv_append(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* k,
+                           const float* v);
+/* Device-pointer form on `stream` (NULL: the context's stream). */
+gmoe_status gmoe_kv_append_async(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* d_k,
+                                 const float* d_v, void* stream);
+/* Rows of the cache as f32: row i of k and v [n x kv_dim] receives position pos[i] of sequence
+ * seqs[i], the key rotated; in 8 bits, what a complete block holds, and the f32 rows of an
+ * incomplete one. Refused when a position is not in the cache. Any order; a row may be read
+ * twice. Synchronous; host pointers. */
+gmoe_status gmoe_kv_read(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const uint32_t* pos, uint32_t n, float* k,
+                         float* v);
+/* Device-pointer form on `stream` (NULL: the context's stream). */
+gmoe_status gmoe_kv_read_async(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const uint32_t* pos, uint32_t n,
+                               float* d_k, float* d_v, void* stream);
+/* Sequence seqs[i] goes back to at most lens[i] positions, in every layer (a layer that is not
+ * longer stays as it is): drafted tokens that were not accepted, an answer asked for again.
+ * Pages past them return to the pool. In 8 bits, positions that are kept of the last
+ * position's block are what they were; of an earlier block that is now incomplete, they are
+ * what it held in 8 bits. Ordered on `stream` (NULL: the context's stream) like the cache's
+ * other calls; returns without waiting. */
+gmoe_status gmoe_kv_truncate(gmoe_kv* kv, const uint32_t* seqs, const uint32_t* lens, uint32_t n, void* stream);
+
 /* ---- expert prediction and prefetch into the slab (predictor/mod.rs, prefetch/mod.rs) ----
  *
  * The reference's ExpertPredictor (predictor/mod.rs:15-134): a first-order Markov model,
