@@ -498,7 +498,8 @@ struct Kv8Job {
   uint32_t pad;
   uint32_t ent[kKv8Block];
 };
-// Consecutive entries of one sequence, from entry i0 and position pos0 on; job: of pos0's block.
+// Consecutive entries of one sequence in one block, from entry i0 and position pos0 on, at most
+// kv8_group_tokens of them; job: of their block.
 struct Kv8Run {
   uint32_t i0, n, pos0, job, table;
 };
@@ -507,6 +508,11 @@ struct Kv8Run {
 struct Kv8Rows {
   uint32_t table, block, i0, r0, n, whole;
 };
+// Positions a part of a row's span has, and how many parts a span needs at most (the first
+// one is the row's own block; the others begin at a block's start).
+constexpr uint32_t kKv8Split = 512;
+constexpr uint32_t kv8_parts(uint32_t span) { return 1 + (span + kKv8Block - 1 + kKv8Split - 1) / kKv8Split; }
+constexpr uint32_t kv8_group_tokens(uint32_t heads) { return 16 / heads; }  // of 16 rows
 constexpr uint32_t kKv8Inline = 64;  // entries, or blocks of a read, carried in the kernel arguments
 struct Kv8Args {
   Kv8Pool p;
@@ -521,6 +527,8 @@ struct Kv8Args {
   const Kv8Job* hjob;  // [njob] in pinned host memory, and the runs; k8_append copies them to
   const Kv8Run* hrun;  //   run for the launches after it
   Kv8Run* run;
+  float* part;         // nparts * n * n_heads * (hd + 2) floats: partial sums (k8_rows)
+  uint32_t nparts;     // own block, then as many splits as the longest span has
   float* own;          // [njob][2][n_kv][16][hd]: the jobs' f32 rows, keys rotated; null: not wanted
   uint32_t njob, nrun;
 };

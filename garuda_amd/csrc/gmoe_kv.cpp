@@ -333,13 +333,14 @@ Kv8Args args8(const gmoe_kv* kv, uint32_t n, const float* q, const float* k, con
 }
 
 // The blocks that a planned call appends to, those of one sequence in position order, and its
-// runs (pages: job_pages, after the commit).
+// groups of rows (pages: job_pages, after the commit).
 void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEntry* ent, std::vector<Kv8Job>& jobs,
                std::vector<Kv8Run>& runs) {
   struct Of {
     uint32_t count = 0, pos0 = 0, job = 0;
   };
   std::vector<Of> of(kv->seqs.size());
+  const uint32_t most = kv8_group_tokens(kv->d.n_heads / kv->d.n_kv_heads);
   for (uint32_t i = 0; i < n; i++) {
     Of& o = of[seqs[i]];
     if (!o.count++) o.pos0 = ent[i].pos;
@@ -363,9 +364,13 @@ void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEn
       }
     }
     jobs[o.job + block - o.pos0 / kKv8Block].ent[row] = i;
-    if (i && ent[i - 1].pages == ent[i].pages) runs.back().n++;
+    if (i && row && ent[i - 1].pages == ent[i].pages && runs.back().n < most) runs.back().n++;
     else runs.push_back(Kv8Run{i, 1, ent[i].pos, o.job + block - o.pos0 / kKv8Block, table});
   }
+}
+
+size_t part8_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nparts) {
+  return (size_t)nparts * n * kv->d.n_heads * (kv->d.head_dim + 2) * 4;
 }
 
 void job_pages(std::vector<Kv8Job>& jobs, const AttnEntry* ent) {
@@ -388,15 +393,16 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   uint8_t* pin = nullptr;
   if (out && distinct) {
     Kv8Inline inl{};
-    const size_t eb = n * sizeof(AttnEntry);
-    if (n > kKv8Inline) {
-      if (gmoe_status s = grow_scratch(kv, eb)) return s;
+    const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
+    a.nparts = kv8_parts(maxspan);
+    if (gmoe_status s = grow_scratch(kv, eb + part8_bytes(kv, n, a.nparts))) return s;
+    if (eb)
       if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
-    }
+    a.part = reinterpret_cast<float*>(kv->scratch + eb);
     commit(kv, layer, seqs, n, ent.data());
     if (pin) {
-      memcpy(pin, ent.data(), eb);
-      KV_TRY(hipMemcpyAsync(kv->scratch, pin, eb, hipMemcpyHostToDevice, st));
+      memcpy(pin, ent.data(), n * sizeof(AttnEntry));
+      KV_TRY(hipMemcpyAsync(kv->scratch, pin, n * sizeof(AttnEntry), hipMemcpyHostToDevice, st));
       a.ent = reinterpret_cast<const AttnEntry*>(kv->scratch);
     } else {
       std::copy(ent.begin(), ent.begin() + n, inl.e);
@@ -408,8 +414,10 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   std::vector<Kv8Run> runs;
   find_jobs(kv, seqs, n, ent.data(), jobs, runs);
   const size_t jb = jobs.size() * sizeof(Kv8Job), rb = runs.size() * sizeof(Kv8Run), o_own = (rb + 255) & ~(size_t)255;
+  const size_t o_part = o_own + jobs.size() * 2 * kKv8Block * kv->kvd * 4;
+  a.nparts = kv8_parts(maxspan);
   if (out)
-    if (gmoe_status s = grow_scratch(kv, o_own + jobs.size() * 2 * kKv8Block * kv->kvd * 4)) return s;
+    if (gmoe_status s = grow_scratch(kv, o_part + part8_bytes(kv, n, a.nparts))) return s;
   if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
   commit(kv, layer, seqs, n, ent.data());
   job_pages(jobs, ent.data());
@@ -422,6 +430,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   if (out) {
     a.run = reinterpret_cast<Kv8Run*>(kv->scratch);
     a.own = reinterpret_cast<float*>(kv->scratch + o_own);
+    a.part = reinterpret_cast<float*>(kv->scratch + o_part);
   }
   KV_TRY(launch_kv8_call(a, st));
   return GMOE_OK;
@@ -753,15 +762,20 @@ void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector
 }
 
 
+// Scratch of a decode step of n sequences over nchunk chunks.
+static size_t step_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nchunk) {
+  return kv->q8 ? part8_bytes(kv, n, kv8_parts(nchunk * kAttnChunk)) : layout(kv, n, nchunk).total;
+}
+
 gmoe_status kv_reserve(gmoe_kv* kv, uint32_t n, uint32_t nchunk) {
   std::lock_guard<std::mutex> g(kv->mu);
   KV_TRY(hipSetDevice(ctx_device(kv->ctx)));
   if (kv->fail_reserves) {
     kv->fail_reserves--;
     return kfail(GMOE_ERR_DEVICE, "attention scratch of %zu bytes: allocation refused (test hook)",
-                 layout(kv, n, nchunk).total);
+                 step_bytes(kv, n, nchunk));
   }
-  return grow_scratch(kv, layout(kv, n, nchunk).total);
+  return grow_scratch(kv, step_bytes(kv, n, nchunk));
 }
 
 const void* kv_scratch_id(gmoe_kv* kv) { return kv->scratch; }
@@ -784,6 +798,9 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
     a.ent = d_ent;
     a.nsl = nsl;
     a.sl_stride = sl_stride;
+    a.part = reinterpret_cast<float*>(kv->scratch);
+    a.nparts = kv8_parts(nchunk * kAttnChunk);
+    if (step_bytes(kv, n, nchunk) > kv->scratch_bytes) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
     KV_TRY(launch_kv8_step(a, Kv8Inline{}, st));
     return GMOE_OK;
   }

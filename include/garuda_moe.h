@@ -422,8 +422,8 @@ gmoe_status gmoe_attention_async(gmoe_kv* kv, uint32_t layer, const uint32_t* se
  * bound the attention of decode steps. Every call on a cache takes either kind.
  *
  * Of one sequence, layer and kv head, a block of 16 positions' keys (values) x is held as
- * integers rint(x * 127 / m), m the largest |x| of the block, and one f32 scale m / 127, and
- * stands for their product; it is held so from the call on that appends its last position.
+ * integers rint(x * (127 * (1 / m))), m the largest |x| of the block (in 64 bits), and one f32
+ * scale m / 127, and stands for their product; it is held so from the call on that appends its last position.
  * The block that a sequence's last position is in is held in f32 besides. A token attends to
  * the positions of its own block as they were given (keys rotated), and to earlier blocks as
  * held in 8 bits, so its context does not depend on how the sequence was cut into calls

@@ -38,7 +38,7 @@ def hold(x: np.ndarray) -> np.ndarray:
         elif m == 0:
             out[:, h] = 0
         else:
-            codes = np.rint(x[:, h].astype(np.float64) * (127.0 / np.float64(m)))
+            codes = np.rint(x[:, h].astype(np.float64) * (127.0 * (1.0 / np.float64(m))))
             out[:, h] = codes.astype(np.float32) * np.float32(np.float64(m) / 127.0)
     return out
 
