@@ -61,13 +61,14 @@ __device__ __forceinline__ float2 pair_of(const float* p, uint32_t j, uint32_t n
   return v;
 }
 
-// The 16 rows kt, vt (in LDS, hs floats apart) of one block and head to codes and scales, by 256
-// threads; red: 8 words of LDS. Every thread calls it after a barrier that follows the rows'.
-__device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const float* vt, uint32_t hs, uint32_t* red) {
-  const uint32_t t = threadIdx.x, n = kKv8Block * p.hd;
-  uint32_t mk = 0, mv = 0;  // as bits: NaN above infinity above every number
-  for (uint32_t x = t; x < n; x += 256) {
-    const uint32_t at = x / p.hd * hs + x % p.hd;
+// The largest magnitudes of a block's 16 key and value rows kt, vt (in LDS, hs floats apart), as
+// bits: a NaN's above infinity's above every number's. red: 8 words of LDS. By 256 threads,
+// after a barrier that follows the rows'.
+__device__ uint2 block_max(const float* kt, const float* vt, uint32_t hd, uint32_t hs, uint32_t* red) {
+  const uint32_t t = threadIdx.x;
+  uint32_t mk = 0, mv = 0;
+  for (uint32_t x = t; x < kKv8Block * hd; x += 256) {
+    const uint32_t at = x / hd * hs + x % hd;
     mk = max(mk, __float_as_uint(kt[at]) & 0x7fffffffu);
     mv = max(mv, __float_as_uint(vt[at]) & 0x7fffffffu);
   }
@@ -80,8 +81,12 @@ __device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const
     red[4 + (t >> 6)] = mv;
   }
   __syncthreads();
-  mk = max(max(red[0], red[1]), max(red[2], red[3]));
-  mv = max(max(red[4], red[5]), max(red[6], red[7]));
+  return make_uint2(max(max(red[0], red[1]), max(red[2], red[3])), max(max(red[4], red[5]), max(red[6], red[7])));
+}
+
+// The block's rows, of maxima m (block_max), to codes and scales.
+__device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const float* vt, uint32_t hs, uint2 m) {
+  const uint32_t t = threadIdx.x;
   // 127 times 1 / m, as a program without a kernel forms it: on a tie (x = m / 2) the product's last
   // bit decides, and the same operations give the same code
   auto inv = [](uint32_t m) { return m == 0 || m >= 0x7f800000u ? 0.0 : 127.0 * (1.0 / (double)__uint_as_float(m)); };
@@ -90,7 +95,7 @@ __device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const
   };
   // a NaN's code is any: its block's scale says so
   auto code = [](float x, double i) { return i == 0.0 ? 128u : (uint32_t)((int)rint((double)x * i) + 128) & 255u; };
-  const double ik = inv(mk), iv = inv(mv);
+  const double ik = inv(m.x), iv = inv(m.y);
   uint8_t* dst = kv8_codes(p, unit);
   for (uint32_t x = t; x < kKv8Block * p.hdp / 4; x += 256) {
     const uint32_t r = x / (p.hdp / 4), d = x % (p.hdp / 4) * 4;
@@ -106,16 +111,17 @@ __device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const
     vd[x] = w;
   }
   if (t == 0) {
-    p.scales[2 * unit] = scale(mk);
-    p.scales[2 * unit + 1] = scale(mv);
+    p.scales[2 * unit] = scale(m.x);
+    p.scales[2 * unit + 1] = scale(m.y);
   }
 }
 
 // Rows of one block and kv head, hs floats apart: those below r0 from the open rows, the next n
-// from k (rotated) and v, row r being entry ent(r); zeros after them.
+// from k (rotated) and v, row r being entry ent(r); zeros after them. ang, if given: the new
+// rows' angles [row][hd / 2].
 template <class F>
 __device__ __forceinline__ void block_rows(const Kv8Args& a, uint32_t table, uint32_t block, uint32_t r0, uint32_t n,
-                                           uint32_t h, float* kt, float* vt, uint32_t hs, F&& ent) {
+                                           uint32_t h, float* kt, float* vt, uint32_t hs, F&& ent, double2* ang = nullptr) {
   const Kv8Pool& p = a.p;
   const uint32_t t = threadIdx.x, hd = p.hd, half = hd / 2;
   const float* old = kv8_open(p, table, h);
@@ -129,6 +135,7 @@ __device__ __forceinline__ void block_rows(const Kv8Args& a, uint32_t table, uin
     const size_t from = (size_t)ent(r) * a.kv_stride + h * hd;
     double cs, sn;
     turn(p.turns[c], block * kKv8Block + r, cs, sn);
+    if (ang) ang[r * half + c] = make_double2(cs, sn);
     const float2 k = pair_of(a.k + from, c, a.nsl, a.sl_stride), v = pair_of(a.v + from, c, a.nsl, a.sl_stride);
     reinterpret_cast<float2*>(kt + r * hs)[c] = rotated(k.x, k.y, cs, sn);
     reinterpret_cast<float2*>(vt + r * hs)[c] = v;
@@ -146,42 +153,54 @@ __device__ void put_open(const Kv8Pool& p, uint32_t table, uint32_t n, uint32_t 
   }
 }
 
-// grid (njob, n_kv), 256 threads: a block of the call's positions, one kv head. The job of a
-// sequence's first block writes the open rows of its last one, after it has read those that
-// were there.
+// grid (njob, n_kv), 256 threads: a block of the call's positions, one kv head and, where the
+// call attends, its query heads, whose turned rows go to a.qr. The job of a sequence's first
+// block writes the open rows of its last one, after it has read those that were there. Copies
+// the call's groups and tiles to the device for the launches after it.
 __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
-  extern __shared__ float lds_f[];
+  extern __shared__ double2 lds_d2[];
   __shared__ uint32_t red[8];
   __shared__ Kv8Job job;
   const Kv8Pool& p = a.p;
-  const uint32_t h = blockIdx.y, t = threadIdx.x, n = kKv8Block * p.hd;
-  float *kt = lds_f, *vt = kt + n;
-  auto rows = [&](uint32_t i) {  // job i, from pinned memory, and its rows
+  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, half = hd / 2, n = kKv8Block * hd;
+  float* kt = reinterpret_cast<float*>(lds_d2 + (a.qr ? kKv8Block * half : 0));
+  float* vt = kt + n;
+  auto rows = [&](uint32_t i, double2* ang) {  // job i, from pinned memory, and its rows
     if (t < sizeof(Kv8Job) / 4) reinterpret_cast<uint32_t*>(&job)[t] = reinterpret_cast<const uint32_t*>(a.hjob + i)[t];
     __syncthreads();
-    block_rows(a, job.table, job.block, job.r0, job.n, h, kt, vt, p.hd, [&](uint32_t r) { return job.ent[r]; });
+    block_rows(a, job.table, job.block, job.r0, job.n, h, kt, vt, hd, [&](uint32_t r) { return job.ent[r]; }, ang);
     __syncthreads();
   };
-  rows(blockIdx.x);
+  rows(blockIdx.x, a.qr ? lds_d2 : nullptr);
   const uint32_t flags = job.flags, last = job.last;
-  if (h == 0 && a.run)
-    for (uint32_t x = blockIdx.x * 256 + t; x < a.nrun; x += gridDim.x * 256) a.run[x] = a.hrun[x];
   if (h == 0 && t == 0 && (flags & kKv8Fresh))
     p.tables[(size_t)job.table * p.ppseq + job.block / (p.bs / kKv8Block)] = job.page;
-  if (a.own) {
+  uint2 m = make_uint2(0, 0);
+  if (a.qr || (flags & kKv8Whole)) m = block_max(kt, vt, hd, hd, red);
+  if (a.qr) {
+    if (h == 0)
+      for (uint32_t x = blockIdx.x * 256 + t; x < a.nrun + a.ntile; x += gridDim.x * 256) a.run[x] = a.hrun[x];
     float* own = a.own + ((size_t)blockIdx.x * 2 * p.n_kv + h) * n;
     for (uint32_t x = t; x < n; x += 256) {
       own[x] = kt[x];
       own[(size_t)p.n_kv * n + x] = vt[x];
     }
+    if (t == 0) a.own_max[(size_t)blockIdx.x * p.n_kv + h] = make_float2(__uint_as_float(m.x), __uint_as_float(m.y));
+    const uint32_t G = a.n_heads / p.n_kv;
+    for (uint32_t x = t; x < job.n * G * half; x += 256) {
+      const uint32_t c = x % half, g = x / half % G, r = job.r0 + x / half / G;
+      const double2 cs = lds_d2[r * half + c];
+      const float* q = a.q + (size_t)job.ent[r] * a.q_stride + (h * G + g) * hd + 2 * c;
+      reinterpret_cast<float2*>(a.qr + ((size_t)job.ent[r] * a.n_heads + h * G + g) * hd)[c] = rotated(q[0], q[1], cs.x, cs.y);
+    }
   }
-  if (flags & kKv8Whole) hold_block(p, kv8_block(p, job.page, job.block, h), kt, vt, p.hd, red);
+  if (flags & kKv8Whole) hold_block(p, kv8_block(p, job.page, job.block, h), kt, vt, hd, m);
   if (!(flags & kKv8First)) return;
   if (last != blockIdx.x) {
     __syncthreads();
-    rows(last);
+    rows(last, nullptr);
   }
-  put_open(p, job.table, job.r0 + job.n, h, kt, vt, p.hd);
+  put_open(p, job.table, job.r0 + job.n, h, kt, vt, hd);
 }
 
 // ---------------------------------------------------------------------------------
@@ -272,13 +291,22 @@ __device__ float uniform_mean(const Kv8Pool& p, uint32_t table, uint32_t h, uint
   return (float)(sum / (double)(pos + 1 - start));
 }
 
-struct Kv8Part {  // partial sums: o [part][n * n_heads][hd], then (max, sum) [part][n * n_heads]
+// Partial sums of the rows of nx groups (or tiles), up to R a kv head: o [part][group][kv head]
+// [R][hd], then (max, sum) [part][group][kv head][R].
+struct Kv8Part {
   float* o;
   float2* ml;
+  uint32_t nx, n_kv, R;
+  __device__ size_t row(uint32_t z, uint32_t x, uint32_t h, uint32_t r) const {
+    return (((size_t)z * nx + x) * n_kv + h) * R + r;
+  }
 };
-__device__ __forceinline__ Kv8Part parts_of(const Kv8Args& a) {
-  float* o = a.part;
-  return {o, reinterpret_cast<float2*>(o + (size_t)a.nparts * a.n * a.n_heads * a.p.hd)};
+__device__ __forceinline__ Kv8Part parts_of(const Kv8Args& a, float* o, uint32_t nparts, uint32_t nx, uint32_t R) {
+  return {o, reinterpret_cast<float2*>(o + (size_t)nparts * nx * a.p.n_kv * R * a.p.hd), nx, a.p.n_kv, R};
+}
+__device__ __forceinline__ Kv8Part rows_parts(const Kv8Args& a, bool step) {
+  const uint32_t G = a.n_heads / a.p.n_kv;
+  return parts_of(a, a.part, a.nparts, step ? a.n : a.nrun, step ? G : kv8_group_tokens(G) * G);
 }
 
 // LDS of k8_rows in floats: queries, the own block's keys and values, its weights and sums, the waves' sums.
@@ -318,10 +346,8 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   const uint32_t own = run.pos0 / kKv8Block * kKv8Block, last = run.pos0 + run.n - 1;
   const uint32_t base = start_of(run.pos0) / kKv8Block * kKv8Block;
   const uint32_t lo = base + (ONE || z == 0 ? 0 : z - 1) * kKv8Split, hi = min(own, lo + kKv8Split);
-  const Kv8Part part = parts_of(a);
-  auto prow = [&](uint32_t r) {  // row r's place in a part
-    return (size_t)z * a.n * a.n_heads + (size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G;
-  };
+  const Kv8Part part = rows_parts(a, STEP);
+  auto prow = [&](uint32_t r) { return part.row(z, x, h, r); };
   if (!ONE && z && lo >= hi) {
     if (t < rows) part.ml[prow(t)] = make_float2(-INFINITY, 0.0f);
     return;
@@ -368,7 +394,9 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   for (uint32_t y = t; y < rows * (HDP / 2); y += 256) {
     const uint32_t r = y / (HDP / 2), c = y % (HDP / 2);
     float2 w = make_float2(0.0f, 0.0f);
-    if (2 * c < hd) {
+    if (!STEP && 2 * c < hd) {
+      w = reinterpret_cast<const float2*>(a.qr + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd)[c];
+    } else if (2 * c < hd) {
       double cs, sn;
       turn(p.turns[c], run.pos0 + r / G, cs, sn);
       const float2 q = pair_of(a.q + (size_t)(run.i0 + r / G) * a.q_stride + (h * G + r % G) * hd, c, a.nsl, a.sl_stride);
@@ -382,7 +410,7 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
       if (e.fresh && h == 0 && t == 0) e.pages[run.pos0 / p.bs] = e.page;  // for the calls after this one
       block_rows(a, run.table, block, r0, 1, h, kt, vt, hs, [&](uint32_t) { return x; });
       __syncthreads();
-      if (r0 == kKv8Block - 1) hold_block(p, kv8_block(p, e.page, block, h), kt, vt, hs, red);
+      if (r0 == kKv8Block - 1) hold_block(p, kv8_block(p, e.page, block, h), kt, vt, hs, block_max(kt, vt, hd, hs, red));
       put_open(p, run.table, r0 + 1, h, kt, vt, hs);
     } else {
       const float* src = a.own + ((size_t)run.job * 2 * p.n_kv + h) * kKv8Block * hd;
@@ -645,16 +673,26 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   }
 }
 
-// grid (n, n_heads), 256 threads: a row's parts joined, threads of several groups taking
+// grid (groups, n_kv R), 256 threads: a row's parts joined, threads of several groups taking
 // every ng-th part for four columns each, the groups then added in order.
 template <bool STEP>
 __global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
   __shared__ float4 go[256];
   __shared__ float gl[256], gm[4];
   const Kv8Pool& p = a.p;
-  const uint32_t i = blockIdx.x, hh = blockIdx.y, t = threadIdx.x, hd = p.hd, q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
-  const size_t rows = (size_t)a.n * a.n_heads, row = (size_t)i * a.n_heads + hh;
-  const Kv8Part part = parts_of(a);
+  const uint32_t x = blockIdx.x, t = threadIdx.x, hd = p.hd, q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
+  const uint32_t G = a.n_heads / p.n_kv;
+  const Kv8Part part = rows_parts(a, STEP);
+  const uint32_t h = blockIdx.y / part.R, r = blockIdx.y % part.R;
+  Kv8Run run;
+  if (STEP) {
+    const AttnEntry e = a.ent ? a.ent[x] : inl.e[x];
+    run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
+  } else {
+    run = a.run[x];
+  }
+  if (r >= run.n * G) return;
+  const size_t rows = (size_t)part.nx * part.n_kv * part.R, row = part.row(0, x, h, r);
   float m = -INFINITY;
   bool bad = false;
   for (uint32_t s = t; s < a.nparts; s += 256) {
@@ -703,32 +741,517 @@ __global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
     }
     o = make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
   } else {
-    const uint32_t h = hh / (a.n_heads / p.n_kv);
-    uint32_t pos, table;
-    const float* vo;
-    if (STEP) {
-      const AttnEntry e = a.ent ? a.ent[i] : inl.e[i];
-      pos = e.pos;
-      table = (uint32_t)((e.pages - p.tables) / p.ppseq);
-      vo = kv8_open(p, table, h) + (size_t)p.n_kv * kKv8Block * hd;
-    } else {
-      uint32_t r = 0;
-      while (i - a.run[r].i0 >= a.run[r].n) r++;
-      const Kv8Run run = a.run[r];
-      pos = run.pos0 + i - run.i0;
-      table = run.table;
-      vo = a.own + (((size_t)run.job * 2 + 1) * p.n_kv + h) * kKv8Block * hd;
-    }
+    const uint32_t pos = run.pos0 + r / G;
+    const float* vo = STEP ? kv8_open(p, run.table, h) + (size_t)p.n_kv * kKv8Block * hd
+                           : a.own + (((size_t)run.job * 2 + 1) * p.n_kv + h) * kKv8Block * hd;
     const uint32_t start = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0;
     float u[4];
-    for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, table, h, start, pos, 4 * t + k, vo, hd);
+    for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, start, pos, 4 * t + k, vo, hd);
     o = make_float4(u[0], u[1], u[2], u[3]);
   }
-  float* dst = a.ctx + row * hd + 4 * t;
+  float* dst = a.ctx + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd + 4 * t;
   dst[0] = o.x;
   dst[1] = o.y;
   dst[2] = o.z;
   dst[3] = o.w;
+}
+
+// ---------------------------------------------------------------------------------
+// Attention of a prompt: tiles of up to 256 (token, query head) rows of one kv head.
+//
+// One workgroup a (kv head, tile, split of the keys), 8 waves of 32 rows. The groups above
+// read a kv head's codes once for 16 rows; here 64 positions at a time go through LDS for
+// 256, converted to fp16 once (16 KB of keys and 16 of values transposed, two buffers: the
+// next tile's codes are in registers while this one's products run). Products as above, on
+// v_mfma_f32_32x32x16_f16: S^T = K Q^T with the rows of A in such an order that a lane's
+// 16 scores of 32 positions are 8 consecutive ones of each of two blocks, its own half of
+// the second product's B operand; O^T = V^T P^T.
+//
+// Split 0 then takes the rows' own blocks, 32 positions at a time: f32 rows, scaled by a power of
+// two for each block, as two fp16 each, three of the four products of two such sums (the
+// fourth is 2^-22 of the first). A row that meets a score that is NaN or +inf, or whose own block
+// has a value that is not finite, is marked and summed again by itself in f32 (row_again).
+//
+// Grid x is the kv head: workgroups go round-robin over the 8 XCDs, so with 8 kv heads a
+// head's codes are read into one XCD's L2.
+// ---------------------------------------------------------------------------------
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float max32(float v) {
+  const LanePair p = xor32_pair(v);
+  return fmaxf(p.a, p.b);
+}
+__device__ __forceinline__ Kv8Part tile_parts(const Kv8Args& a) {
+  return parts_of(a, a.tpart, a.tsplits, a.ntile, kKv8TileRows);
+}
+
+template <int NS>
+__global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
+  constexpr uint32_t HDP = 32 * NS, KS = HDP / 16, NP = NS / 2, CH = HDP / 8;  // CH: 16-byte columns of a key row
+  constexpr uint32_t KX = CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;             // keys' column x is at x ^ (key % KX)
+  constexpr uint32_t KB = 64 * HDP * 2, BUF = 2 * KB;                          // bytes of a tile's keys; of a buffer
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
+  __shared__ float2 sc[2][4];
+  const Kv8Pool& p = a.p;
+  const uint32_t h = blockIdx.x, x = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
+  const uint32_t lane = t & 63, l32 = lane & 31, hf = lane >> 5;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane(v); };
+  const Kv8Run* T = a.run + a.nrun + x;
+  const uint32_t i0 = uni(T->i0), ntok = uni(T->n), pos0 = uni(T->pos0), table = uni(T->table), job0 = uni(T->job);
+  const uint32_t rows = ntok * G, last = pos0 + ntok - 1;
+  auto start_of = [&](uint32_t pos) { return a.window && pos + 1 > a.window ? pos + 1 - a.window : 0; };
+  auto own_of = [](uint32_t pos) { return pos / kKv8Block * kKv8Block; };
+  const uint32_t base = own_of(start_of(pos0)), lo = base + z * a.tkeys, hi = min(own_of(last), lo + a.tkeys);
+  const uint32_t row = 32 * wave + l32, rr = min(row, rows - 1), pos = pos0 + rr / G;
+  const uint32_t start = start_of(pos), own = own_of(pos);
+  const Kv8Part part = tile_parts(a);
+  const size_t prow = part.row(z, x, h, row);  // 256 rows a kv head
+  const bool mine = row < rows, busy = 32 * wave < rows;
+  if (z && lo >= hi) {
+    if (mine && hf == 0) part.ml[prow] = make_float2(-INFINITY, 0.0f);
+    return;
+  }
+  // what the wave's rows attend to of the held blocks: from its first row's start to its last row's own block
+  const uint32_t pw0 = pos0 + min(32 * wave, rows - 1) / G, pw1 = pos0 + min(32 * wave + 31, rows - 1) / G;
+  const uint32_t w_lo = start_of(pw0), w_hi = min(own_of(pw1), hi), w_in0 = start_of(pw1), w_in1 = min(own_of(pw0), hi);
+
+  // the thread's 16 bytes of codes of a tile: block sb, column sx of its HDP; the page looked up
+  // a tile ahead
+  const uint32_t sb = t / HDP, sx = t % HDP;
+  const bool stage = sb < 4;
+  auto find = [&](uint32_t kb) {
+    const uint32_t b = min(kb + kKv8Block * min(sb, 3u), hi - 1) / kKv8Block;
+    return kv8_block(p, kv8_page(p, table, b), b, h);
+  };
+  uint4 kc, vc;
+  float2 sv2;
+  auto load = [&](size_t unit) {
+    const uint8_t* c = p.codes + unit * (2 * kKv8Block * HDP) + sx * 16;
+    if (stage) {
+      kc = *reinterpret_cast<const uint4*>(c);
+      vc = *reinterpret_cast<const uint4*>(c + kKv8Block * HDP);
+      sv2 = reinterpret_cast<const float2*>(p.scales)[unit];
+    }
+  };
+  uint32_t krow, kcol;  // the keys' row in its block and first 16-byte column
+  if (NS % 2 && sx >= 64 * NP) {
+    krow = (sx - 64 * NP) / 2;
+    kcol = 8 * NP + 2 * (sx % 2);
+  } else {
+    krow = sx % 64 / 4;
+    kcol = 8 * (sx / 64) + 2 * (sx % 4);
+  }
+  auto store = [&](uint32_t b) {
+    if (!stage) return;
+    uint8_t* buf = lds + b * BUF;
+    const uint32_t key = kKv8Block * sb + krow;
+    *reinterpret_cast<f16x8*>(buf + key * HDP * 2 + ((kcol ^ (key % KX)) * 16)) = codes8(kc.x, kc.y);
+    *reinterpret_cast<f16x8*>(buf + key * HDP * 2 + (((kcol + 1) ^ (key % KX)) * 16)) = codes8(kc.z, kc.w);
+    *reinterpret_cast<f16x8*>(buf + KB + sx * 128 + (((2 * sb) ^ (sx % 8)) * 16)) = codes8(vc.x, vc.y);
+    *reinterpret_cast<f16x8*>(buf + KB + sx * 128 + (((2 * sb + 1) ^ (sx % 8)) * 16)) = codes8(vc.z, vc.w);
+    if (sx == 0) sc[b][sb] = sv2;
+  };
+  const bool any = lo < hi;
+  size_t unit = 0;
+  if (any) {
+    unit = find(lo);
+    load(unit);
+    unit = find(lo + 64);
+  }
+  // queries: the wave's B operand
+  f16x8 qh[KS], ql[KS];
+  float cq;
+  bool odd;
+  {
+    const float* q = a.qr + ((size_t)(i0 + rr / G) * a.n_heads + h * G + rr % G) * hd;
+    float4 v[KS][2];
+    float m = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++)
+#pragma unroll
+      for (uint32_t y = 0; y < 2; y++) {
+        const uint32_t d = 16 * s + 8 * hf + 4 * y;
+        v[s][y] = d < hd ? *reinterpret_cast<const float4*>(q + d) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (float f : {v[s][y].x, v[s][y].y, v[s][y].z, v[s][y].w}) {
+          m = fmaxf(m, fabsf(f));
+          top = max(top, __float_as_uint(f) & 0x7fffffffu);
+        }
+      }
+    m = max32(m);
+    odd = max32(top >= 0x7f800000u ? 1.0f : 0.0f) != 0.0f;
+    const int eq = odd ? 0 : pow2_of(m);
+    const float up = pow2(9 - eq);
+    cq = a.scale * kLog2e * pow2(max(eq - 9, -126));
+#pragma unroll
+    for (uint32_t s = 0; s < KS; s++) {
+      float f[8] = {v[s][0].x * up, v[s][0].y * up, v[s][0].z * up, v[s][0].w * up,
+                    v[s][1].x * up, v[s][1].y * up, v[s][1].z * up, v[s][1].w * up};
+      if (odd)
+        for (int y = 0; y < 8; y++) f[y] = 0.0f;
+      split8(f, qh[s], ql[s]);
+    }
+  }
+  f32x16 o[NS], zero;
+#pragma unroll
+  for (int r = 0; r < 16; r++) zero[r] = 0.0f;
+#pragma unroll
+  for (int d = 0; d < NS; d++) o[d] = zero;
+  float M = -INFINITY, L = 0.0f;
+  int ev = -100;
+  // a lane's key of the MFMA's row l32: 8 consecutive ones of a block to a half
+  const uint32_t arow = 16 * (l32 / 16) + 8 * (l32 / 4 % 2) + 4 * (l32 / 8 % 2) + l32 % 4;
+  // scores s (scaled, masked), each eight of a block whose values have the scale svn, to weights and the row's sums
+  auto soften = [&](float* s, int n, const float* svn, float* w) {
+    float mt = -INFINITY;
+    int en = ev;
+    for (int y = 0; y < n; y++) {
+      odd |= __builtin_amdgcn_classf(s[y], 0x203);
+      mt = fmaxf(mt, s[y]);
+    }
+    for (int y = 0; y < n / 8; y++) en = max(en, pow2_of(svn[y]));
+    mt = fmaxf(M, max32(mt) - 14.0f);
+    const float mu = mt == -INFINITY ? 0.0f : mt;
+    float f = __builtin_amdgcn_exp2f(M - mu);
+    L *= f;
+    f *= pow2(max(ev - en, -126));
+    if (__ballot(f != 1.0f)) {
+#pragma unroll
+      for (int d = 0; d < NS; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] *= f;
+    }
+    M = mt;
+    ev = en;
+    const float un = pow2(-en);
+    float sum = 0.0f;
+    for (int y = 0; y < n; y++) {
+      const float pv = __builtin_amdgcn_exp2f(s[y] - mu);
+      sum += pv;
+      w[y] = pv * (svn[y / 8] * un);
+    }
+    L += sum;
+  };
+  if (any) store(0);
+  __syncthreads();
+  uint32_t buf = 0;
+  for (uint32_t kb = lo; kb < hi; kb += 64, buf ^= 1) {
+    const bool more = kb + 64 < hi;
+    if (more) {
+      load(unit);
+      if (kb + 128 < hi) unit = find(kb + 128);
+    }
+    if (busy && kb < w_hi && kb + 64 > w_lo) {
+      const uint8_t* kbuf = lds + buf * BUF;
+      float s[32], w[32], svn[4];
+#pragma unroll
+      for (uint32_t b = 0; b < 2; b++) {
+        f32x16 acc = zero;
+#pragma unroll
+        for (uint32_t st = 0; st < KS; st++) {
+          const uint32_t key = 32 * b + arow;
+          const f16x8 kf = *reinterpret_cast<const f16x8*>(kbuf + key * HDP * 2 + (((2 * st + hf) ^ (key % KX)) * 16));
+          acc = mfma32(kf, ql[st], acc);
+          acc = mfma32(kf, qh[st], acc);
+        }
+#pragma unroll
+        for (uint32_t y = 0; y < 2; y++) {
+          const float2 c = sc[buf][2 * b + y];
+          svn[2 * b + y] = c.y;
+          const float ck = c.x * cq;
+#pragma unroll
+          for (uint32_t r = 0; r < 8; r++) s[16 * b + 8 * y + r] = acc[8 * y + r] * ck;
+        }
+      }
+      if (kb < w_in0 || kb + 64 > w_in1) {  // positions that some row of the wave does not attend to
+        const uint32_t top = min(own, hi);
+#pragma unroll
+        for (uint32_t y = 0; y < 4; y++) {
+          const uint32_t k0 = kb + 16 * y;
+          if (k0 >= top || k0 + 16 <= start) svn[y] = 0.0f;
+#pragma unroll
+          for (uint32_t r = 0; r < 8; r++) {
+            const uint32_t pk = k0 + 8 * hf + r;
+            if (pk < start || pk >= top) s[8 * y + r] = -INFINITY;
+          }
+        }
+      }
+      soften(s, 32, svn, w);
+#pragma unroll
+      for (uint32_t y = 0; y < 4; y++) {
+        f16x8 wh, wl;
+        split8(w + 8 * y, wh, wl);
+#pragma unroll
+        for (uint32_t d = 0; d < NS; d++) {
+          const uint32_t dr = 32 * d + l32;
+          const f16x8 vf = *reinterpret_cast<const f16x8*>(kbuf + KB + dr * 128 + (((2 * y + hf) ^ (dr % 8)) * 16));
+          o[d] = mfma32(vf, wl, o[d]);
+          o[d] = mfma32(vf, wh, o[d]);
+        }
+      }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  if (z == 0) {
+    // the rows' own blocks, two at a time: planes of keys [2][32][HDP], of values transposed [2][HDP][32]
+    constexpr uint32_t PK = 32 * HDP * 2, PV = HDP * 32 * 2;
+    const uint32_t b_end = last / kKv8Block;
+    for (uint32_t b0 = pos0 / kKv8Block; b0 <= b_end; b0 += 2) {
+      float2 up[2];  // powers of two: keys and values below 2^10
+      float svn[2], skn[2];
+      bool wild[2];
+#pragma unroll
+      for (uint32_t y = 0; y < 2; y++) {
+        const uint32_t job = job0 + min(b0 + y, b_end) - pos0 / kKv8Block;
+        const float2 m = a.own_max[(size_t)job * p.n_kv + h];
+        wild[y] = !(fabsf(m.x) < INFINITY) || !(fabsf(m.y) < INFINITY);
+        const int ek = wild[y] ? 0 : pow2_of(m.x), em = wild[y] ? 0 : pow2_of(m.y);
+        up[y] = make_float2(pow2(9 - ek), pow2(9 - em));
+        skn[y] = pow2(max(ek - 9, -126));
+        svn[y] = pow2(max(em - 9, -126));
+      }
+      auto src = [&](uint32_t y, uint32_t kv) {  // rows of block b0 + y
+        const uint32_t job = job0 + min(b0 + y, b_end) - pos0 / kKv8Block;
+        return a.own + (((size_t)job * 2 + kv) * p.n_kv + h) * kKv8Block * hd;
+      };
+      __syncthreads();
+      for (uint32_t it = t; it < 32 * (HDP / 4); it += 512) {
+        const uint32_t key = it / (HDP / 4), d = it % (HDP / 4) * 4;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (d < hd && !(key < 16 ? wild[0] : wild[1])) v = *reinterpret_cast<const float4*>(src(key / 16, 0) + key % 16 * hd + d);
+        const float u = key < 16 ? up[0].x : up[1].x;
+        const float f[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
+        uint8_t* dst = lds + key * HDP * 2 + (((d / 8) ^ (key % KX)) * 16 + 8 * (d / 4 % 2));
+        f16x2 hi2[2], lo2[2];
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          hi2[y] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(f[2 * y], f[2 * y + 1]));
+          lo2[y][0] = (_Float16)(f[2 * y] - (float)hi2[y][0]);
+          lo2[y][1] = (_Float16)(f[2 * y + 1] - (float)hi2[y][1]);
+        }
+        *reinterpret_cast<u32x2*>(dst) = u32x2{__builtin_bit_cast(uint32_t, hi2[0]), __builtin_bit_cast(uint32_t, hi2[1])};
+        *reinterpret_cast<u32x2*>(dst + PK) = u32x2{__builtin_bit_cast(uint32_t, lo2[0]), __builtin_bit_cast(uint32_t, lo2[1])};
+      }
+      for (uint32_t it = t; it < 16 * (HDP / 4); it += 512) {
+        const uint32_t kp = it % 16, d = it / 16 * 4, key = 2 * kp;
+        float4 v0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v1 = v0;
+        if (d < hd && !(key < 16 ? wild[0] : wild[1])) {  // 0 times a NaN would reach the other block's rows
+          const float* s = src(key / 16, 1) + key % 16 * hd + d;
+          v0 = *reinterpret_cast<const float4*>(s);
+          v1 = *reinterpret_cast<const float4*>(s + hd);
+        }
+        const float u = key < 16 ? up[0].y : up[1].y;
+        const float f[4][2] = {{v0.x * u, v1.x * u}, {v0.y * u, v1.y * u}, {v0.z * u, v1.z * u}, {v0.w * u, v1.w * u}};
+#pragma unroll
+        for (uint32_t y = 0; y < 4; y++) {
+          const f16x2 hi2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(f[y][0], f[y][1]));
+          const f16x2 lo2 = {(_Float16)(f[y][0] - (float)hi2[0]), (_Float16)(f[y][1] - (float)hi2[1])};
+          uint8_t* dst = lds + 2 * PK + (d + y) * 64 + (((key / 8) ^ ((d + y) / 2 % 4)) * 16 + 2 * (key % 8));
+          *reinterpret_cast<uint32_t*>(dst) = __builtin_bit_cast(uint32_t, hi2);
+          *reinterpret_cast<uint32_t*>(dst + PV) = __builtin_bit_cast(uint32_t, lo2);
+        }
+      }
+      __syncthreads();
+      const uint32_t k0 = b0 * kKv8Block;
+      if (busy && k0 <= pw1 && k0 + 32 > own_of(pw0)) {
+        f32x16 acc = zero;
+#pragma unroll
+        for (uint32_t st = 0; st < KS; st++) {
+          const uint8_t* at = lds + arow * HDP * 2 + (((2 * st + hf) ^ (arow % KX)) * 16);
+          const f16x8 kh = *reinterpret_cast<const f16x8*>(at), kl = *reinterpret_cast<const f16x8*>(at + PK);
+          acc = mfma32(kl, qh[st], acc);
+          acc = mfma32(kh, ql[st], acc);
+          acc = mfma32(kh, qh[st], acc);
+        }
+        float s[16], w[16], sn[2];
+#pragma unroll
+        for (uint32_t y = 0; y < 2; y++) {
+          const bool at = own == k0 + 16 * y;
+          odd |= at && wild[y];
+          sn[y] = at && !wild[y] ? svn[y] : 0.0f;
+          const float ck = skn[y] * cq;
+#pragma unroll
+          for (uint32_t r = 0; r < 8; r++) {
+            const uint32_t pk = k0 + 16 * y + 8 * hf + r;
+            s[8 * y + r] = at && !wild[y] && pk <= pos && pk >= start ? acc[8 * y + r] * ck : -INFINITY;
+          }
+        }
+        soften(s, 16, sn, w);
+#pragma unroll
+        for (uint32_t y = 0; y < 2; y++) {
+          f16x8 wh, wl;
+          split8(w + 8 * y, wh, wl);
+#pragma unroll
+          for (uint32_t d = 0; d < NS; d++) {
+            const uint32_t dr = 32 * d + l32;
+            const uint8_t* at = lds + 2 * PK + dr * 64 + (((2 * y + hf) ^ (dr / 2 % 4)) * 16);
+            const f16x8 vh = *reinterpret_cast<const f16x8*>(at), vl = *reinterpret_cast<const f16x8*>(at + PV);
+            o[d] = mfma32(vl, wh, o[d]);
+            o[d] = mfma32(vh, wl, o[d]);
+            o[d] = mfma32(vh, wh, o[d]);
+          }
+        }
+      }
+    }
+  }
+  {
+    const LanePair l = xor32_pair(L);
+    L = l.a + l.b;
+  }
+  odd = max32(odd ? 1.0f : 0.0f) != 0.0f;
+  const float fo = pow2(ev);
+  if (mine) {
+    if (hf == 0) part.ml[prow] = make_float2(odd ? __uint_as_float(kBadRow) : M, L);
+#pragma unroll
+    for (uint32_t d = 0; d < NS; d++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t c = 32 * d + 8 * j + 4 * hf;
+        if (c < hd)
+          *reinterpret_cast<float4*>(part.o + prow * hd + c) =
+              make_float4(o[d][4 * j] * fo, o[d][4 * j + 1] * fo, o[d][4 * j + 2] * fo, o[d][4 * j + 3] * fo);
+      }
+  }
+}
+
+// One row again, by the workgroup, in f32: 64 positions at a time, four threads a score. ls: 64
+// floats, po: 256 float4 of LDS. Threads t < hd / 4 return the row's columns 4 t .. 4 t + 3.
+__device__ float4 row_again(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r, float* ls, float4* po) {
+  const Kv8Pool& p = a.p;
+  const uint32_t t = threadIdx.x, lane = t & 63, hd = p.hd, G = a.n_heads / p.n_kv, pos = run.pos0 + r / G;
+  const uint32_t start = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0, own = pos / kKv8Block * kKv8Block;
+  const float* q = a.qr + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd;
+  const uint32_t job = run.job + pos / kKv8Block - run.pos0 / kKv8Block;
+  const float* ko = a.own + ((size_t)job * 2 * p.n_kv + h) * kKv8Block * hd;
+  const float* vo = ko + (size_t)p.n_kv * kKv8Block * hd;
+  const uint32_t q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
+  float M = -INFINITY, L = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  bool uniform = false;
+  for (uint32_t c0 = start / kKv8Block * kKv8Block; c0 <= pos && !uniform; c0 += 64) {
+    const uint32_t pk = c0 + t / 4;
+    float s = 0.0f;
+    const bool in = pk >= start && pk <= pos;
+    if (in) {
+      const size_t u = pk < own ? kv8_block(p, kv8_page(p, run.table, pk / kKv8Block), pk / kKv8Block, h) : 0;
+      for (uint32_t d = t % 4; d < hd; d += 4)
+        s = fmaf(q[d], pk < own ? (float)((int)kv8_codes(p, u)[kv8_key(p.hdp, pk % kKv8Block, d)] - 128) : ko[(pk - own) * hd + d], s);
+      if (pk < own) s *= p.scales[2 * u];
+    }
+    s += __shfl_xor(s, 1, 64);
+    s += __shfl_xor(s, 2, 64);
+    __syncthreads();
+    if (t % 4 == 0) ls[t / 4] = in ? s * (a.scale * kLog2e) : -INFINITY;
+    __syncthreads();
+    const float v = ls[lane];
+    if (__ballot(v != v || v == INFINITY)) uniform = true;  // every wave sees the same scores
+    const float mc = wave64_max(v);
+    if (uniform || mc == -INFINITY) continue;
+    const float mn = fmaxf(M, mc), f = __builtin_amdgcn_exp2f(M - mn), pv = __builtin_amdgcn_exp2f(v - mn);
+    M = mn;
+    L = L * f + wave64_sum(pv);
+    __syncthreads();
+    if (t < 64) ls[t] = pv;
+    __syncthreads();
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    if (g < ng)
+      for (uint32_t j = g; j < 64; j += ng) {
+        const uint32_t pj = c0 + j;
+        if (pj < start || pj > pos) continue;
+        const float w = ls[j];
+        float4 b;
+        if (pj < own) {
+          const size_t u = kv8_block(p, kv8_page(p, run.table, pj / kKv8Block), pj / kKv8Block, h);
+          const uint8_t* cv = kv8_codes(p, u) + kKv8Block * p.hdp + pj % kKv8Block;
+          const float sv = p.scales[2 * u + 1];
+          auto at = [&](uint32_t d) { return (float)((int)cv[d * kKv8Block] - 128) * sv; };
+          b = make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
+        } else {
+          b = *reinterpret_cast<const float4*>(vo + (pj - own) * hd + 4 * c);
+        }
+        o = make_float4(fmaf(w, b.x, o.x), fmaf(w, b.y, o.y), fmaf(w, b.z, o.z), fmaf(w, b.w, o.w));
+      }
+  }
+  if (uniform || M == -INFINITY) {
+    if (t >= q4) return o;
+    float u[4];
+    for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, start, pos, 4 * t + k, vo, hd);
+    return make_float4(u[0], u[1], u[2], u[3]);
+  }
+  __syncthreads();
+  po[t] = o;
+  __syncthreads();
+  if (t < q4) {
+    for (uint32_t k = 1; k < ng; k++) {
+      const float4 b = po[k * q4 + t];
+      o = make_float4(o.x + b.x, o.y + b.y, o.z + b.z, o.w + b.w);
+    }
+    o = make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
+  }
+  return o;
+}
+
+// grid (tiles, n_kv, ceil(256 / rows a workgroup)), 256 threads: the splits of a tile's rows
+// joined, a thread per four columns of a row.
+__global__ void __launch_bounds__(256) k8_join_tile(Kv8Args a) {
+  __shared__ float4 po[256];
+  __shared__ float ls[64];
+  __shared__ uint32_t marks[8];
+  const Kv8Pool& p = a.p;
+  const uint32_t x = blockIdx.x, h = blockIdx.y, t = threadIdx.x, hd = p.hd, q4 = hd / 4, rpw = 256 / q4, G = a.n_heads / p.n_kv;
+  const Kv8Run run = a.run[a.nrun + x];
+  const Kv8Part part = tile_parts(a);
+  const uint32_t r0 = blockIdx.z * rpw, r = r0 + t / q4, c = t % q4, rows = run.n * G;
+  if (r0 >= rows) return;
+  const bool mine = t / q4 < rpw && r < rows;
+  auto dst = [&](uint32_t r) { return a.ctx + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd; };
+  auto put = [&](float* d, float4 v) {
+    d[0] = v.x;
+    d[1] = v.y;
+    d[2] = v.z;
+    d[3] = v.w;
+  };
+  if (t < 8) marks[t] = 0;
+  __syncthreads();
+  if (mine) {
+    const size_t step = (size_t)part.nx * part.n_kv * part.R, row = part.row(0, x, h, r);
+    float m = -INFINITY, l = 0.0f;
+    bool again = false;
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t s = 0; s < a.tsplits; s++) {
+      const float v = part.ml[s * step + row].x;
+      again |= v != v;
+      m = fmaxf(m, v);
+    }
+    again |= m == -INFINITY;
+    if (!again) {
+      for (uint32_t s = 0; s < a.tsplits; s++) {
+        const float2 v = part.ml[s * step + row];
+        if (!(v.x > -INFINITY)) continue;
+        const float f = __builtin_amdgcn_exp2f(v.x - m);
+        const float4 w = reinterpret_cast<const float4*>(part.o + (s * step + row) * hd)[c];
+        l += v.y * f;
+        o = make_float4(o.x + w.x * f, o.y + w.y * f, o.z + w.z * f, o.w + w.w * f);
+      }
+      put(dst(r) + 4 * c, make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
+    } else if (c == 0) {
+      atomicOr(&marks[t / q4 / 32], 1u << (t / q4 % 32));
+    }
+  }
+  __syncthreads();
+  for (uint32_t k = 0; k < 8; k++)
+    for (uint32_t left = marks[k]; left; left &= left - 1) {
+      const uint32_t r1 = r0 + 32 * k + __builtin_ctz(left);
+      const float4 v = row_again(a, run, h, r1, ls, po);
+      if (t < q4) put(dst(r1) + 4 * t, v);
+      __syncthreads();
+    }
 }
 
 // grid (chunks, n_kv), 256 threads: rows of one block, from its codes or from the open rows.
@@ -775,20 +1298,19 @@ __global__ void __launch_bounds__(256) k8_reopen(Kv8Pool p, Kv8RowsInline inl) {
 bool overlaps(const float* a, size_t na, const float* b, size_t nb) { return a < b + nb && b < a + na; }
 
 // One workgroup a group and kv head: everything before the own block fits one part, and no
-// other workgroup's input lies under the context.
+// other workgroup's input lies under the context (a call reads its own in the launch before).
 bool one_part(const Kv8Args& a, bool step) {
   const size_t n = a.n, qd = (size_t)a.n_heads * a.p.hd, kvd = (size_t)a.p.n_kv * a.p.hd;
   const size_t more = a.nsl > 1 ? (a.nsl - 1) * a.sl_stride : 0;
   auto over = [&](const float* p, size_t width, size_t stride) {
     return overlaps(a.ctx, n * qd, p, (n - 1) * stride + width + more);
   };
-  if (a.nparts != 2 || over(a.q, qd, a.q_stride)) return false;
-  return !step || (!over(a.k, kvd, a.kv_stride) && !over(a.v, kvd, a.kv_stride));
+  if (a.nparts != 2) return false;
+  return !step || (!over(a.q, qd, a.q_stride) && !over(a.k, kvd, a.kv_stride) && !over(a.v, kvd, a.kv_stride));
 }
 
 template <int NS, bool STEP>
 void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
-  const bool one = one_part(a, STEP);
   // what 16 rows of the widest heads of this build take, set once; a call asks for its own rows'
   static const bool set = [] {
     const int most = (int)kv8_rows_lds(32 * NS, 32 * NS, 16);
@@ -796,12 +1318,13 @@ void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
            hipFuncSetAttribute((const void*)k8_rows<NS, STEP, false>, hipFuncAttributeMaxDynamicSharedMemorySize, most) == hipSuccess;
   }();
   (void)set;
-  const uint32_t G = a.n_heads / a.p.n_kv, rows = STEP ? G : kv8_group_tokens(G) * G;
+  const bool one = one_part(a, STEP);
+  const uint32_t G = a.n_heads / a.p.n_kv, rows = STEP ? G : kv8_group_tokens(G) * G, nx = STEP ? a.n : a.nrun;
   const uint32_t lds = kv8_rows_lds(a.p.hd, a.p.hdp, rows);
-  const dim3 grid(STEP ? a.n : a.nrun, a.p.n_kv, one ? 1 : a.nparts);
+  const dim3 grid(nx, a.p.n_kv, one ? 1 : a.nparts);
   auto kernel = one ? k8_rows<NS, STEP, true> : k8_rows<NS, STEP, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, inl);
-  if (!one) hipLaunchKernelGGL(k8_join<STEP>, dim3(a.n, a.n_heads), dim3(256), 0, st, a, inl);
+  if (!one) hipLaunchKernelGGL(k8_join<STEP>, dim3(nx, a.p.n_kv * rows), dim3(256), 0, st, a, inl);
 }
 
 template <bool STEP>
@@ -822,9 +1345,21 @@ hipError_t launch_rows_of(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) { return launch_rows_of<true>(a, inl, st); }
 
 hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
-  hipLaunchKernelGGL(k8_append, dim3(a.njob, a.p.n_kv), dim3(256), 2 * kKv8Block * a.p.hd * 4, st, a);
+  const uint32_t lds = 2 * kKv8Block * a.p.hd * 4 + (a.qr ? kKv8Block * a.p.hd / 2 * 16 : 0);
+  hipLaunchKernelGGL(k8_append, dim3(a.njob, a.p.n_kv), dim3(256), lds, st, a);
   if (!a.ctx) return hipGetLastError();
-  return launch_rows_of<false>(a, Kv8Inline{}, st);
+  if (a.ntile) {
+    const dim3 grid(a.p.n_kv, a.ntile, a.tsplits);
+    switch (a.p.hdp / 32) {
+      case 1: hipLaunchKernelGGL(k8_tile<1>, grid, dim3(512), 0, st, a); break;
+      case 2: hipLaunchKernelGGL(k8_tile<2>, grid, dim3(512), 0, st, a); break;
+      case 3: hipLaunchKernelGGL(k8_tile<3>, grid, dim3(512), 0, st, a); break;
+      default: hipLaunchKernelGGL(k8_tile<4>, grid, dim3(512), 0, st, a); break;
+    }
+    const uint32_t rpw = 256 / (a.p.hd / 4);
+    hipLaunchKernelGGL(k8_join_tile, dim3(a.ntile, a.p.n_kv, (kKv8TileRows + rpw - 1) / rpw), dim3(256), 0, st, a);
+  }
+  return a.nrun ? launch_rows_of<false>(a, Kv8Inline{}, st) : hipGetLastError();
 }
 
 hipError_t launch_kv8_read(const Kv8Pool& p, const Kv8Rows* rows, const Kv8RowsInline& inl, uint32_t nrows, float* k,

@@ -498,8 +498,8 @@ struct Kv8Job {
   uint32_t pad;
   uint32_t ent[kKv8Block];
 };
-// Consecutive entries of one sequence in one block, from entry i0 and position pos0 on, at most
-// kv8_group_tokens of them; job: of their block.
+// Consecutive entries of one sequence, from entry i0 and position pos0 on; job: of pos0's block.
+// A group: at most kv8_group_tokens of one block. A tile: at most kv8_tile_tokens.
 struct Kv8Run {
   uint32_t i0, n, pos0, job, table;
 };
@@ -513,6 +513,8 @@ struct Kv8Rows {
 constexpr uint32_t kKv8Split = 512;
 constexpr uint32_t kv8_parts(uint32_t span) { return 1 + (span + kKv8Block - 1 + kKv8Split - 1) / kKv8Split; }
 constexpr uint32_t kv8_group_tokens(uint32_t heads) { return 16 / heads; }  // of 16 rows
+constexpr uint32_t kKv8TileRows = 256, kKv8TileHd = 128;  // and the widest heads that tiles take
+constexpr uint32_t kv8_tile_tokens(uint32_t heads) { return kKv8TileRows / heads; }
 constexpr uint32_t kKv8Inline = 64;  // entries, or blocks of a read, carried in the kernel arguments
 struct Kv8Args {
   Kv8Pool p;
@@ -525,12 +527,16 @@ struct Kv8Args {
   uint64_t sl_stride;
   float* ctx;
   const Kv8Job* hjob;  // [njob] in pinned host memory, and the runs; k8_append copies them to
-  const Kv8Run* hrun;  //   run for the launches after it
+  const Kv8Run* hrun;  //   run for the launches after it: nrun groups, then ntile tiles
   Kv8Run* run;
-  float* part;         // nparts * n * n_heads * (hd + 2) floats: partial sums (k8_rows)
-  uint32_t nparts;     // own block, then as many splits as the longest span has
-  float* own;          // [njob][2][n_kv][16][hd]: the jobs' f32 rows, keys rotated; null: not wanted
-  uint32_t njob, nrun;
+  uint32_t njob, nrun, ntile;
+  float* qr;           // [n][n_heads * hd] rotated queries; null: the call only appends
+  float* own;          // [njob][2][n_kv][16][hd]: the jobs' f32 rows, keys rotated,
+  float2* own_max;     //   and [njob][n_kv] their largest magnitudes (keys, values)
+  float* part;         // partial sums of the groups' rows (kv8_part_floats): the own block,
+  uint32_t nparts;     //   then as many splits as the longest span has
+  float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions
+  uint32_t tsplits, tkeys;
 };
 struct Kv8Inline {
   AttnEntry e[kKv8Inline];

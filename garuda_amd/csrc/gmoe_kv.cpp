@@ -332,15 +332,14 @@ Kv8Args args8(const gmoe_kv* kv, uint32_t n, const float* q, const float* k, con
   return a;
 }
 
-// The blocks that a planned call appends to, those of one sequence in position order, and its
-// groups of rows (pages: job_pages, after the commit).
+// The blocks that a planned call appends to, those of one sequence in position order (pages:
+// job_pages, after the commit), and its runs: consecutive entries of one sequence.
 void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEntry* ent, std::vector<Kv8Job>& jobs,
                std::vector<Kv8Run>& runs) {
   struct Of {
     uint32_t count = 0, pos0 = 0, job = 0;
   };
   std::vector<Of> of(kv->seqs.size());
-  const uint32_t most = kv8_group_tokens(kv->d.n_heads / kv->d.n_kv_heads);
   for (uint32_t i = 0; i < n; i++) {
     Of& o = of[seqs[i]];
     if (!o.count++) o.pos0 = ent[i].pos;
@@ -363,14 +362,51 @@ void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEn
         jobs.push_back(j);
       }
     }
-    jobs[o.job + block - o.pos0 / kKv8Block].ent[row] = i;
-    if (i && row && ent[i - 1].pages == ent[i].pages && runs.back().n < most) runs.back().n++;
-    else runs.push_back(Kv8Run{i, 1, ent[i].pos, o.job + block - o.pos0 / kKv8Block, table});
+    const uint32_t job = o.job + block - o.pos0 / kKv8Block;
+    jobs[job].ent[row] = i;
+    if (i && ent[i - 1].pages == ent[i].pages) runs.back().n++;
+    else runs.push_back(Kv8Run{i, 1, ent[i].pos, job, table});
   }
 }
 
-size_t part8_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nparts) {
-  return (size_t)nparts * n * kv->d.n_heads * (kv->d.head_dim + 2) * 4;
+// The runs cut into groups of at most 16 rows, or tiles of at most 256 where a run has rows for
+// a quarter of one: with fewer, most of a tile's waves idle while the groups read the cache
+// a few times.
+constexpr uint32_t kKv8TileMin = 64;
+void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
+  const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
+  for (const Kv8Run& r : runs) {
+    const bool tile = kv->d.head_dim <= kKv8TileHd && (uint64_t)r.n * G >= kKv8TileMin;
+    for (uint32_t at = 0, m; at < r.n; at += m) {
+      const uint32_t pos = r.pos0 + at;
+      m = std::min(r.n - at, tile ? kv8_tile_tokens(G) : std::min(kv8_group_tokens(G), kKv8Block - pos % kKv8Block));
+      (tile ? tiles : groups).push_back(Kv8Run{r.i0 + at, m, pos, r.job + pos / kKv8Block - r.pos0 / kKv8Block, r.table});
+    }
+  }
+}
+
+// Positions of a tile's split: the tiles' keys are split over workgroups until the call has
+// about one a CU, each split keeping at least four steps of 64 positions.
+constexpr uint32_t kKv8TileWgs = 256;
+uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_t* splits) {
+  uint32_t span = 1;
+  for (const Kv8Run& t : tiles) {
+    const uint32_t w = kv->d.sliding_window, from = w && t.pos0 + 1 > w ? t.pos0 + 1 - w : 0;
+    span = std::max(span, (t.pos0 + t.n - 1) / kKv8Block * kKv8Block - std::min(t.pos0, from) / kKv8Block * kKv8Block);
+  }
+  const uint32_t steps = (span + 63) / 64, wgs = (uint32_t)tiles.size() * kv->d.n_kv_heads;
+  const uint32_t ns = std::max(1u, std::min((kKv8TileWgs + wgs - 1) / wgs, steps / 4));
+  const uint32_t keys = (steps + ns - 1) / ns * 64;
+  *splits = (span + keys - 1) / keys;
+  return keys;
+}
+
+// Scratch of the partial sums of nx groups (tiles) of R rows a kv head.
+size_t part8_bytes(const gmoe_kv* kv, size_t nx, uint32_t R, uint32_t nparts) {
+  return (nparts * nx * kv->d.n_kv_heads * R * (kv->d.head_dim + 2) * 4 + 255) & ~(size_t)255;
+}
+size_t step8_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nparts) {
+  return part8_bytes(kv, n, kv->d.n_heads / kv->d.n_kv_heads, nparts);
 }
 
 void job_pages(std::vector<Kv8Job>& jobs, const AttnEntry* ent) {
@@ -395,7 +431,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     Kv8Inline inl{};
     const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
     a.nparts = kv8_parts(maxspan);
-    if (gmoe_status s = grow_scratch(kv, eb + part8_bytes(kv, n, a.nparts))) return s;
+    if (gmoe_status s = grow_scratch(kv, eb + step8_bytes(kv, n, a.nparts))) return s;
     if (eb)
       if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
     a.part = reinterpret_cast<float*>(kv->scratch + eb);
@@ -411,26 +447,51 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     return GMOE_OK;
   }
   std::vector<Kv8Job> jobs;
-  std::vector<Kv8Run> runs;
+  std::vector<Kv8Run> runs, groups, tiles;
   find_jobs(kv, seqs, n, ent.data(), jobs, runs);
-  const size_t jb = jobs.size() * sizeof(Kv8Job), rb = runs.size() * sizeof(Kv8Run), o_own = (rb + 255) & ~(size_t)255;
-  const size_t o_part = o_own + jobs.size() * 2 * kKv8Block * kv->kvd * 4;
-  a.nparts = kv8_parts(maxspan);
-  if (out)
-    if (gmoe_status s = grow_scratch(kv, o_part + part8_bytes(kv, n, a.nparts))) return s;
-  if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {  // of the scratch
+    const size_t o = at;
+    at += (bytes + 255) & ~(size_t)255;
+    return o;
+  };
+  size_t o_run = 0, o_qr = 0, o_own = 0, o_max = 0, o_part = 0, o_tpart = 0;
+  if (out) {
+    cut_runs(kv, runs, groups, tiles);
+    a.nrun = (uint32_t)groups.size();
+    a.ntile = (uint32_t)tiles.size();
+    if (a.ntile) a.tkeys = tile_split(kv, tiles, &a.tsplits);
+    if (a.nrun) {
+      uint32_t span = 1;  // a group's first token has the longest way back of its tokens, or as long a one
+      for (const Kv8Run& g : groups) span = std::max(span, ent[g.i0 + g.n - 1].pos + 1 - ent[g.i0].start);
+      a.nparts = kv8_parts(span);
+    }
+    const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
+    o_run = take((groups.size() + tiles.size()) * sizeof(Kv8Run));
+    o_qr = take((size_t)n * kv->d.n_heads * kv->d.head_dim * 4);
+    o_own = take(jobs.size() * 2 * kKv8Block * kv->kvd * 4);
+    o_max = take(jobs.size() * kv->d.n_kv_heads * sizeof(float2));
+    o_part = take(part8_bytes(kv, groups.size(), kv8_group_tokens(G) * G, a.nparts));
+    o_tpart = take(part8_bytes(kv, tiles.size(), kKv8TileRows, a.tsplits));
+    if (gmoe_status s = grow_scratch(kv, at)) return s;
+  }
+  const size_t jb = jobs.size() * sizeof(Kv8Job), gb = groups.size() * sizeof(Kv8Run), tb = tiles.size() * sizeof(Kv8Run);
+  if (gmoe_status s = take_pinned(kv, jb + gb + tb, st, &pin)) return s;
   commit(kv, layer, seqs, n, ent.data());
   job_pages(jobs, ent.data());
   memcpy(pin, jobs.data(), jb);
-  memcpy(pin + jb, runs.data(), rb);
+  if (gb) memcpy(pin + jb, groups.data(), gb);
+  if (tb) memcpy(pin + jb + gb, tiles.data(), tb);
   a.hjob = reinterpret_cast<const Kv8Job*>(pin);
   a.hrun = reinterpret_cast<const Kv8Run*>(pin + jb);
   a.njob = (uint32_t)jobs.size();
-  a.nrun = (uint32_t)runs.size();
   if (out) {
-    a.run = reinterpret_cast<Kv8Run*>(kv->scratch);
+    a.run = reinterpret_cast<Kv8Run*>(kv->scratch + o_run);
+    a.qr = reinterpret_cast<float*>(kv->scratch + o_qr);
     a.own = reinterpret_cast<float*>(kv->scratch + o_own);
+    a.own_max = reinterpret_cast<float2*>(kv->scratch + o_max);
     a.part = reinterpret_cast<float*>(kv->scratch + o_part);
+    a.tpart = reinterpret_cast<float*>(kv->scratch + o_tpart);
   }
   KV_TRY(launch_kv8_call(a, st));
   return GMOE_OK;
@@ -764,7 +825,7 @@ void kv_restore(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const std::vector
 
 // Scratch of a decode step of n sequences over nchunk chunks.
 static size_t step_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nchunk) {
-  return kv->q8 ? part8_bytes(kv, n, kv8_parts(nchunk * kAttnChunk)) : layout(kv, n, nchunk).total;
+  return kv->q8 ? step8_bytes(kv, n, kv8_parts(nchunk * kAttnChunk)) : layout(kv, n, nchunk).total;
 }
 
 gmoe_status kv_reserve(gmoe_kv* kv, uint32_t n, uint32_t nchunk) {
