@@ -17,6 +17,8 @@
 // span, as with a cache in f32.
 #include "gmoe_device.h"
 
+#include <type_traits>
+
 namespace gmoe {
 
 namespace {
@@ -41,6 +43,8 @@ __device__ __forceinline__ float* kv8_open(const Kv8Pool& p, uint32_t table, uin
   return p.open + ((size_t)table * 2 * p.n_kv + h) * kKv8Block * p.hd;
 }
 
+constexpr uint32_t kv8_pad(uint32_t hd) { return hd + 4; }  // floats between rows in LDS: 16 rows' columns on all banks
+
 __device__ __forceinline__ void turn(double turns, uint32_t pos, double& c, double& s) {
   double t = (double)pos * turns;
   t -= rint(t);
@@ -51,41 +55,107 @@ __device__ __forceinline__ float2 rotated(float x, float y, double c, double s) 
   return make_float2((float)(a * c - b * s), (float)(a * s + b * c));
 }
 
-// Elements 2j and 2j + 1 of p: sums of nsl slices in slice order.
-__device__ __forceinline__ float2 pair_of(const float* p, uint32_t j, uint32_t nsl, uint64_t stride) {
-  float2 v = make_float2(p[2 * j], p[2 * j + 1]);
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows of the caller's: any float's alignment
+__device__ __forceinline__ float4 load4(const float* p) {
+  const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
+  return make_float4(v.x, v.y, v.z, v.w);
+}
+// Four elements from p on: sums of nsl slices in slice order.
+__device__ __forceinline__ float4 four_of(const float* p, uint32_t nsl, uint64_t stride) {
+  float4 v = load4(p);
   for (uint32_t g = 1; g < nsl; g++) {
-    v.x += p[g * stride + 2 * j];
-    v.y += p[g * stride + 2 * j + 1];
+    const float4 w = load4(p + g * stride);
+    v = make_float4(v.x + w.x, v.y + w.y, v.z + w.z, v.w + w.w);
   }
   return v;
 }
-
-// The largest magnitudes of a block's 16 key and value rows kt, vt (in LDS, hs floats apart), as
-// bits: a NaN's above infinity's above every number's. red: 8 words of LDS. By 256 threads,
-// after a barrier that follows the rows'.
-__device__ uint2 block_max(const float* kt, const float* vt, uint32_t hd, uint32_t hs, uint32_t* red) {
-  const uint32_t t = threadIdx.x;
-  uint32_t mk = 0, mv = 0;
-  for (uint32_t x = t; x < kKv8Block * hd; x += 256) {
-    const uint32_t at = x / hd * hs + x % hd;
-    mk = max(mk, __float_as_uint(kt[at]) & 0x7fffffffu);
-    mv = max(mv, __float_as_uint(vt[at]) & 0x7fffffffu);
-  }
-  for (int o = 32; o; o >>= 1) {
-    mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
-    mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
-  }
-  if ((t & 63) == 0) {
-    red[t >> 6] = mk;
-    red[4 + (t >> 6)] = mv;
-  }
-  __syncthreads();
-  return make_uint2(max(max(red[0], red[1]), max(red[2], red[3])), max(max(red[4], red[5]), max(red[6], red[7])));
+// Elements 4c .. 4c + 3 of a head's row at position pos, turned.
+__device__ __forceinline__ float4 turned(const Kv8Pool& p, float4 v, uint32_t c, uint32_t pos) {
+  double cs[2], sn[2];
+  for (uint32_t i = 0; i < 2; i++) turn(p.turns[2 * c + i], pos, cs[i], sn[i]);
+  const float2 a = rotated(v.x, v.y, cs[0], sn[0]), b = rotated(v.z, v.w, cs[1], sn[1]);
+  return make_float4(a.x, a.y, b.x, b.y);
 }
 
-// The block's rows, of maxima m (block_max), to codes and scales.
-__device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const float* vt, uint32_t hs, uint2 m) {
+// The rows of one block and kv head in a thread's registers, 256 threads: float4 i of the keys'
+// [16][HDP] then the values', i = t + 256 y. All loads are in flight together (one after another they
+// were most of a short call).
+template <int NS>
+struct BlockRows {
+  static constexpr uint32_t Q4 = 8 * NS;  // float4 of a row
+  float4 v[NS];
+  static __device__ uint32_t value(uint32_t i) { return i / (16 * Q4); }
+  static __device__ uint32_t row(uint32_t i) { return i / Q4 % 16; }
+  static __device__ uint32_t col(uint32_t i) { return i % Q4; }
+
+  // Rows below r0 from the open rows, the next n from k and v (keys not yet turned), row r being
+  // entry ent(r); zeros after them and past the head's width.
+  template <class F>
+  __device__ __forceinline__ void load(const Kv8Args& a, uint32_t table, uint32_t r0, uint32_t n, uint32_t h, F&& ent) {
+    const Kv8Pool& p = a.p;
+    const float* old = kv8_open(p, table, h);
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      const uint32_t i = threadIdx.x + 256 * y, r = row(i), c = col(i);
+      v[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (4 * c >= p.hd || r >= r0 + n) continue;
+      if (r < r0) v[y] = *reinterpret_cast<const float4*>(old + (size_t)value(i) * p.n_kv * kKv8Block * p.hd + r * p.hd + 4 * c);
+      else v[y] = four_of((value(i) ? a.v : a.k) + (size_t)ent(r) * a.kv_stride + h * p.hd + 4 * c, a.nsl, a.sl_stride);
+    }
+  }
+  __device__ __forceinline__ void turn_keys(const Kv8Pool& p, uint32_t block, uint32_t r0, uint32_t n) {
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      const uint32_t i = threadIdx.x + 256 * y, r = row(i), c = col(i);
+      if (!value(i) && 4 * c < p.hd && r >= r0 && r < r0 + n) v[y] = turned(p, v[y], c, block * kKv8Block + r);
+    }
+  }
+  // to LDS, rows hs floats apart (hs at least HDP)
+  __device__ __forceinline__ void put(float* kt, float* vt, uint32_t hs) const {
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      const uint32_t i = threadIdx.x + 256 * y;
+      *reinterpret_cast<float4*>((value(i) ? vt : kt) + row(i) * hs + 4 * col(i)) = v[y];
+    }
+  }
+  // the first n rows to [2][n_kv][16][hd] at to (of kv head 0)
+  __device__ __forceinline__ void put_global(const Kv8Pool& p, float* to, uint32_t h, uint32_t n) const {
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      const uint32_t i = threadIdx.x + 256 * y, r = row(i), c = col(i);
+      if (r < n && 4 * c < p.hd)
+        *reinterpret_cast<float4*>(to + (((size_t)value(i) * p.n_kv + h) * kKv8Block + r) * p.hd + 4 * c) = v[y];
+    }
+  }
+  // the largest magnitudes of keys and values, as bits: a NaN's above infinity's above every
+  // number's. red: 8 words of LDS.
+  __device__ __forceinline__ uint2 largest(uint32_t* red) const {
+    uint32_t mk = 0, mv = 0;
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      uint32_t m = 0;
+      for (float f : {v[y].x, v[y].y, v[y].z, v[y].w}) m = max(m, __float_as_uint(f) & 0x7fffffffu);
+      if (value(threadIdx.x + 256 * y)) mv = max(mv, m);
+      else mk = max(mk, m);
+    }
+    for (int o = 32; o; o >>= 1) {
+      mk = max(mk, (uint32_t)__shfl_xor((int)mk, o, 64));
+      mv = max(mv, (uint32_t)__shfl_xor((int)mv, o, 64));
+    }
+    const uint32_t t = threadIdx.x;
+    if ((t & 63) == 0) {
+      red[t >> 6] = mk;
+      red[4 + (t >> 6)] = mv;
+    }
+    __syncthreads();
+    return make_uint2(max(max(red[0], red[1]), max(red[2], red[3])), max(max(red[4], red[5]), max(red[6], red[7])));
+  }
+};
+
+// A block's 16 rows (in LDS, hs floats apart), of largest magnitudes m, to codes and scales.
+template <int NS>
+__device__ __forceinline__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const float* vt, uint32_t hs, uint2 m) {
+  constexpr uint32_t HDP = 32 * NS, W = kKv8Block * HDP / 4;  // words of the keys', and of the values' codes
   const uint32_t t = threadIdx.x;
   // 127 times 1 / m, as a program without a kernel forms it: on a tie (x = m / 2) the product's last
   // bit decides, and the same operations give the same code
@@ -97,17 +167,23 @@ __device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const
   auto code = [](float x, double i) { return i == 0.0 ? 128u : (uint32_t)((int)rint((double)x * i) + 128) & 255u; };
   const double ik = inv(m.x), iv = inv(m.y);
   uint8_t* dst = kv8_codes(p, unit);
-  for (uint32_t x = t; x < kKv8Block * p.hdp / 4; x += 256) {
-    const uint32_t r = x / (p.hdp / 4), d = x % (p.hdp / 4) * 4;
+#pragma unroll
+  for (uint32_t y = 0; y < W; y += 256) {
+    const uint32_t x = y + t, r = x / (HDP / 4), d = x % (HDP / 4) * 4;
+    if (W % 256 && x >= W) break;
     uint32_t w = 0;
-    for (uint32_t b = 0; b < 4; b++) w |= (d + b < p.hd ? code(kt[r * hs + d + b], ik) : 128u) << 8 * b;
-    *reinterpret_cast<uint32_t*>(dst + kv8_key(p.hdp, r, d)) = w;
+#pragma unroll
+    for (uint32_t b = 0; b < 4; b++) w |= code(kt[r * hs + d + b], ik) << 8 * b;  // zeros past the head's width
+    *reinterpret_cast<uint32_t*>(dst + kv8_key(HDP, r, d)) = w;
   }
-  uint32_t* vd = reinterpret_cast<uint32_t*>(dst + kKv8Block * p.hdp);
-  for (uint32_t x = t; x < kKv8Block * p.hdp / 4; x += 256) {
-    const uint32_t d = x / 4, r = x % 4 * 4;
+  uint32_t* vd = reinterpret_cast<uint32_t*>(dst + kKv8Block * HDP);
+#pragma unroll
+  for (uint32_t y = 0; y < W; y += 256) {
+    const uint32_t x = y + t, d = x / 4, r = x % 4 * 4;
+    if (W % 256 && x >= W) break;
     uint32_t w = 0;
-    for (uint32_t b = 0; b < 4; b++) w |= (d < p.hd ? code(vt[(r + b) * hs + d], iv) : 128u) << 8 * b;
+#pragma unroll
+    for (uint32_t b = 0; b < 4; b++) w |= code(vt[(r + b) * hs + d], iv) << 8 * b;
     vd[x] = w;
   }
   if (t == 0) {
@@ -116,91 +192,79 @@ __device__ void hold_block(const Kv8Pool& p, size_t unit, const float* kt, const
   }
 }
 
-// Rows of one block and kv head, hs floats apart: those below r0 from the open rows, the next n
-// from k (rotated) and v, row r being entry ent(r); zeros after them. ang, if given: the new
-// rows' angles [row][hd / 2].
-template <class F>
-__device__ __forceinline__ void block_rows(const Kv8Args& a, uint32_t table, uint32_t block, uint32_t r0, uint32_t n,
-                                           uint32_t h, float* kt, float* vt, uint32_t hs, F&& ent, double2* ang = nullptr) {
-  const Kv8Pool& p = a.p;
-  const uint32_t t = threadIdx.x, hd = p.hd, half = hd / 2;
-  const float* old = kv8_open(p, table, h);
-  for (uint32_t x = t; x < r0 * hd; x += 256) {
-    const uint32_t at = x / hd * hs + x % hd;
-    kt[at] = old[x];
-    vt[at] = old[(size_t)p.n_kv * kKv8Block * hd + x];
-  }
-  for (uint32_t x = t; x < n * half; x += 256) {
-    const uint32_t r = r0 + x / half, c = x % half;
-    const size_t from = (size_t)ent(r) * a.kv_stride + h * hd;
-    double cs, sn;
-    turn(p.turns[c], block * kKv8Block + r, cs, sn);
-    if (ang) ang[r * half + c] = make_double2(cs, sn);
-    const float2 k = pair_of(a.k + from, c, a.nsl, a.sl_stride), v = pair_of(a.v + from, c, a.nsl, a.sl_stride);
-    reinterpret_cast<float2*>(kt + r * hs)[c] = rotated(k.x, k.y, cs, sn);
-    reinterpret_cast<float2*>(vt + r * hs)[c] = v;
-  }
-  for (uint32_t x = t + (r0 + n) * hd; x < kKv8Block * hd; x += 256) kt[x / hd * hs + x % hd] = vt[x / hd * hs + x % hd] = 0.0f;
-}
-// The first n rows to the open rows.
-__device__ void put_open(const Kv8Pool& p, uint32_t table, uint32_t n, uint32_t h, const float* kt, const float* vt,
-                         uint32_t hs) {
-  float* to = kv8_open(p, table, h);
-  for (uint32_t x = threadIdx.x; x < n * p.hd; x += 256) {
-    const uint32_t at = x / p.hd * hs + x % p.hd;
-    to[x] = kt[at];
-    to[(size_t)p.n_kv * kKv8Block * p.hd + x] = vt[at];
-  }
-}
-
-// grid (njob, n_kv), 256 threads: a block of the call's positions, one kv head and, where the
-// call attends, its query heads, whose turned rows go to a.qr. The job of a sequence's first
-// block writes the open rows of its last one, after it has read those that were there. Copies
-// the call's groups and tiles to the device for the launches after it.
+// grid (njob, n_kv, 1 + ceil(G / 4) where the call attends), 256 threads: a block of the call's
+// positions and one kv head's keys and values (z 0), or up to four of its query heads, whose
+// turned rows go to a.qr. The job of a sequence's first block writes the open rows of its last
+// one, after it has read those that were there. Copies the call's groups and tiles to the
+// device for the launches after it.
+template <int NS>
 __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
-  extern __shared__ double2 lds_d2[];
+  constexpr uint32_t HS = kv8_pad(32 * NS), Q4 = 8 * NS;
+  __shared__ __attribute__((aligned(16))) float kt[kKv8Block * HS], vt[kKv8Block * HS];
   __shared__ uint32_t red[8];
   __shared__ Kv8Job job;
   const Kv8Pool& p = a.p;
-  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, half = hd / 2, n = kKv8Block * hd;
-  float* kt = reinterpret_cast<float*>(lds_d2 + (a.qr ? kKv8Block * half : 0));
-  float* vt = kt + n;
-  auto rows = [&](uint32_t i, double2* ang) {  // job i, from pinned memory, and its rows
+  const uint32_t h = blockIdx.y, t = threadIdx.x;
+  auto take = [&](uint32_t i) {  // job i, from pinned memory
     if (t < sizeof(Kv8Job) / 4) reinterpret_cast<uint32_t*>(&job)[t] = reinterpret_cast<const uint32_t*>(a.hjob + i)[t];
     __syncthreads();
-    block_rows(a, job.table, job.block, job.r0, job.n, h, kt, vt, hd, [&](uint32_t r) { return job.ent[r]; }, ang);
-    __syncthreads();
   };
-  rows(blockIdx.x, a.qr ? lds_d2 : nullptr);
+  take(blockIdx.x);
+  if (blockIdx.z) {
+    const uint32_t G = a.n_heads / p.n_kv, g0 = 4 * (blockIdx.z - 1), ng = min(G - g0, 4u);
+    float4 q[2 * NS];  // float4 t + 256 y of [ng][16][HDP], in flight together
+    auto at = [&](uint32_t y, uint32_t& g, uint32_t& r, uint32_t& c) {
+      const uint32_t i = t + 256 * y;
+      c = i % Q4;
+      r = i / Q4 % 16;
+      g = i / Q4 / 16;
+      return g < ng && r >= job.r0 && r < job.r0 + job.n && 4 * c < p.hd;
+    };
+#pragma unroll
+    for (uint32_t y = 0; y < 2 * NS; y++) {
+      uint32_t g, r, c;
+      if (at(y, g, r, c)) q[y] = load4(a.q + (size_t)job.ent[r] * a.q_stride + (h * G + g0 + g) * p.hd + 4 * c);
+    }
+    // a thread's floats of one row and column in several heads share their angles
+#pragma unroll
+    for (uint32_t y = 0; y < 2 * NS; y++) {
+      uint32_t g, r, c;
+      if (at(y, g, r, c))
+        *reinterpret_cast<float4*>(a.qr + ((size_t)job.ent[r] * a.n_heads + h * G + g0 + g) * p.hd + 4 * c) =
+            turned(p, q[y], c, job.block * kKv8Block + r);
+    }
+    return;
+  }
   const uint32_t flags = job.flags, last = job.last;
   if (h == 0 && t == 0 && (flags & kKv8Fresh))
     p.tables[(size_t)job.table * p.ppseq + job.block / (p.bs / kKv8Block)] = job.page;
-  uint2 m = make_uint2(0, 0);
-  if (a.qr || (flags & kKv8Whole)) m = block_max(kt, vt, hd, hd, red);
-  if (a.qr) {
-    if (h == 0)
-      for (uint32_t x = blockIdx.x * 256 + t; x < a.nrun + a.ntile; x += gridDim.x * 256) a.run[x] = a.hrun[x];
-    float* own = a.own + ((size_t)blockIdx.x * 2 * p.n_kv + h) * n;
-    for (uint32_t x = t; x < n; x += 256) {
-      own[x] = kt[x];
-      own[(size_t)p.n_kv * n + x] = vt[x];
+  if (h == 0 && a.qr)
+    for (uint32_t x = blockIdx.x * 256 + t; x < a.nrun + a.ntile; x += gridDim.x * 256) a.run[x] = a.hrun[x];
+  BlockRows<NS> rows;
+  auto get = [&] {
+    rows.load(a, job.table, job.r0, job.n, h, [&](uint32_t r) { return job.ent[r]; });
+    rows.turn_keys(p, job.block, job.r0, job.n);
+  };
+  get();
+  if (a.qr || (flags & kKv8Whole)) {
+    const uint2 m = rows.largest(red);
+    if (a.qr) {
+      rows.put_global(p, a.own + (size_t)blockIdx.x * 2 * p.n_kv * kKv8Block * p.hd, h, kKv8Block);
+      if (t == 0) a.own_max[(size_t)blockIdx.x * p.n_kv + h] = make_float2(__uint_as_float(m.x), __uint_as_float(m.y));
     }
-    if (t == 0) a.own_max[(size_t)blockIdx.x * p.n_kv + h] = make_float2(__uint_as_float(m.x), __uint_as_float(m.y));
-    const uint32_t G = a.n_heads / p.n_kv;
-    for (uint32_t x = t; x < job.n * G * half; x += 256) {
-      const uint32_t c = x % half, g = x / half % G, r = job.r0 + x / half / G;
-      const double2 cs = lds_d2[r * half + c];
-      const float* q = a.q + (size_t)job.ent[r] * a.q_stride + (h * G + g) * hd + 2 * c;
-      reinterpret_cast<float2*>(a.qr + ((size_t)job.ent[r] * a.n_heads + h * G + g) * hd)[c] = rotated(q[0], q[1], cs.x, cs.y);
+    if (flags & kKv8Whole) {
+      rows.put(kt, vt, HS);
+      __syncthreads();
+      hold_block<NS>(p, kv8_block(p, job.page, job.block, h), kt, vt, HS, m);
     }
   }
-  if (flags & kKv8Whole) hold_block(p, kv8_block(p, job.page, job.block, h), kt, vt, hd, m);
   if (!(flags & kKv8First)) return;
   if (last != blockIdx.x) {
     __syncthreads();
-    rows(last, nullptr);
+    take(last);
+    get();
   }
-  put_open(p, job.table, job.r0 + job.n, h, kt, vt, hd);
+  rows.put_global(p, p.open + (size_t)job.table * 2 * p.n_kv * kKv8Block * p.hd, h, job.r0 + job.n);
 }
 
 // ---------------------------------------------------------------------------------
@@ -237,20 +301,31 @@ __device__ __forceinline__ f16x8 codes8(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(f16x8, u32x4{code_pair(lo, 0x04010400u), code_pair(lo, 0x04030402u),
                                          code_pair(hi, 0x04010400u), code_pair(hi, 0x04030402u)});
 }
-// Eight values as two fp16 each: the first truncated, the second what it leaves, to nearest
-// (2^-22 of the value). By the conversion's own builtin: a plain cast of a product is folded
-// into one instruction that rounds the product once, and what is left of the product's f32
-// value then belongs to another first half.
+// Two values as two fp16 each: the first to nearest, the second what it leaves, truncated (within
+// 2^-21 of the value, of either sign). The value is made opaque first: a product's conversion may be
+// folded into one instruction that rounds the product once, and what is left of the product's
+// f32 value then belongs to another first half. `one` is 1, opaque too, so that the subtraction
+// is a v_fma_mix_f32, which takes the half as it stands.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  float one = 1.0f;
+  asm("" : "+v"(x), "+v"(y), "+s"(one));
+  const f16x2 h = __builtin_convertvector((f32x2{x, y}), f16x2);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -one, x),
+                                                               __builtin_fmaf((float)h[1], -one, y)));
+}
 __device__ __forceinline__ void split8(const float* x, f16x8& hi, f16x8& lo) {
+  u32x4 h, l;
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    const f16x2 h = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(x[i], x[i + 1]));
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      hi[i + j] = h[j];
-      lo[i + j] = (_Float16)(x[i + j] - (float)h[j]);
-    }
+  for (int i = 0; i < 4; i++) {
+    uint32_t a, b;
+    split2(x[2 * i], x[2 * i + 1], a, b);
+    h[i] = a;
+    l[i] = b;
   }
+  hi = __builtin_bit_cast(f16x8, h);
+  lo = __builtin_bit_cast(f16x8, l);
 }
 __device__ __forceinline__ f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -309,33 +384,74 @@ __device__ __forceinline__ Kv8Part rows_parts(const Kv8Args& a, bool step) {
   return parts_of(a, a.part, a.nparts, step ? a.n : a.nrun, step ? G : kv8_group_tokens(G) * G);
 }
 
-// LDS of k8_rows in floats: queries, the own block's keys and values, its weights and sums, the waves' sums.
-constexpr uint32_t kv8_pad(uint32_t hd) { return hd + 4; }
-uint32_t kv8_rows_lds(uint32_t hd, uint32_t hdp, uint32_t rows) {
-  return (16 * kv8_pad(hdp) + 2 * kKv8Block * kv8_pad(hd) + 16 * 16 + rows * kv8_pad(hd) + 4 * rows * kv8_pad(hdp)) * 4;
+// LDS of k8_rows: queries, the own block's keys and values, its weights and sums, the waves' sums.
+uint32_t kv8_rows_lds(uint32_t hdp, uint32_t rows) {
+  return ((16 + 2 * kKv8Block + rows + 4 * rows) * kv8_pad(hdp) + 16 * 16) * 4;
 }
 
-// STEP: group x is entry x, and the token is appended here. ONE: one workgroup takes both
+// Workgroup i of a step: its entry and part, the entries' parts laid end to end (so that no workgroup
+// is launched for a part that a shorter sequence does not have). Each lane counts one entry's.
+// Returns false past the last.
+__device__ __forceinline__ bool step_part(const Kv8Args& a, const Kv8Inline& inl, uint32_t i, uint32_t& x, uint32_t& z,
+                                          AttnEntry& e) {
+  const uint32_t lane = threadIdx.x & 63;
+  for (uint32_t e0 = 0; e0 < a.n; e0 += 64) {
+    AttnEntry mine{};
+    uint32_t n = 0;
+    if (e0 + lane < a.n) {
+      mine = a.ent ? a.ent[e0 + lane] : inl.e[e0 + lane];
+      n = kv8_parts_of(mine.pos, mine.start);
+    }
+    uint32_t sum = n;  // inclusive prefix
+#pragma unroll
+    for (uint32_t o = 1; o < 64; o *= 2) {
+      const uint32_t v = (uint32_t)__shfl_up((int)sum, o, 64);
+      if (lane >= o) sum += v;
+    }
+    const uint64_t past = __ballot(sum > i);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      x = e0 + l;
+      z = i - (uint32_t)__builtin_amdgcn_readlane((int)(sum - n), l);
+      const uint64_t pages = (uint64_t)mine.pages;
+      e.pages = (uint32_t*)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(pages >> 32), l) << 32 |
+                            (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)pages, l));
+      e.pos = (uint32_t)__builtin_amdgcn_readlane((int)mine.pos, l);
+      e.start = (uint32_t)__builtin_amdgcn_readlane((int)mine.start, l);
+      e.page = (uint32_t)__builtin_amdgcn_readlane((int)mine.page, l);
+      e.fresh = (uint32_t)__builtin_amdgcn_readlane((int)mine.fresh, l);
+      return true;
+    }
+    i -= (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+  }
+  return false;
+}
+
+// STEP: groups are entries, and the token is appended here. ONE: one workgroup takes both
 // the own block and what is before it (at most kKv8Split positions), and writes the context.
+// grid: (groups, n_kv, parts), in a step without ONE (parts of all entries, n_kv).
 template <int NS, bool STEP, bool ONE>
 __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8Inline inl) {
-  constexpr uint32_t HDP = 32 * NS, NP = NS / 2, QS = kv8_pad(HDP);
+  constexpr uint32_t HDP = 32 * NS, NP = NS / 2, QS = kv8_pad(HDP), Q4 = HDP / 4;
   extern __shared__ float4 lds_v4[];
   __shared__ uint32_t red[8];
   __shared__ float own_m[16], own_l[16], wm[4][16], wl[4][16];
   const Kv8Pool& p = a.p;
-  const uint32_t x = blockIdx.x, h = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
+  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
   const uint32_t lane = t & 63, n16 = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  uint32_t x = blockIdx.x, z = blockIdx.z;
   Kv8Run run;
   AttnEntry e{};
   if (STEP) {
-    e = a.ent ? a.ent[x] : inl.e[x];
+    if (ONE) e = a.ent ? a.ent[x] : inl.e[x];
+    else if (!step_part(a, inl, blockIdx.x, x, z, e)) return;
     run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
   } else {
     run = a.run[x];
   }
-  const uint32_t rows = run.n * G, hs = kv8_pad(hd);
+  constexpr uint32_t hs = QS;
+  const uint32_t rows = run.n * G;
   float* qs = reinterpret_cast<float*>(lds_v4);  // [16][QS]
   float* kt = qs + 16 * QS;                      // [16][hs], then the values
   float* vt = kt + kKv8Block * hs;
@@ -348,7 +464,7 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   const uint32_t lo = base + (ONE || z == 0 ? 0 : z - 1) * kKv8Split, hi = min(own, lo + kKv8Split);
   const Kv8Part part = rows_parts(a, STEP);
   auto prow = [&](uint32_t r) { return part.row(z, x, h, r); };
-  if (!ONE && z && lo >= hi) {
+  if (!ONE && z && lo >= hi) {  // a call's group without that part
     if (t < rows) part.ml[prow(t)] = make_float2(-INFINITY, 0.0f);
     return;
   }
@@ -390,34 +506,57 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
     load_k();
     load_v();
   }
-  // queries, turned
-  for (uint32_t y = t; y < rows * (HDP / 2); y += 256) {
-    const uint32_t r = y / (HDP / 2), c = y % (HDP / 2);
-    float2 w = make_float2(0.0f, 0.0f);
-    if (!STEP && 2 * c < hd) {
-      w = reinterpret_cast<const float2*>(a.qr + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd)[c];
-    } else if (2 * c < hd) {
-      double cs, sn;
-      turn(p.turns[c], run.pos0 + r / G, cs, sn);
-      const float2 q = pair_of(a.q + (size_t)(run.i0 + r / G) * a.q_stride + (h * G + r % G) * hd, c, a.nsl, a.sl_stride);
-      w = rotated(q.x, q.y, cs, sn);
+  // queries, turned (a call's were in the launch before)
+  constexpr int QN = (16 * Q4 + 255) / 256;
+  float4 qv[QN];
+  auto q_at = [&](int y, uint32_t& r, uint32_t& c) {
+    const uint32_t i = t + 256 * y;
+    r = i / Q4;
+    c = i % Q4;
+    return r < rows;
+  };
+#pragma unroll
+  for (int y = 0; y < QN; y++) {
+    uint32_t r, c;
+    qv[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (!q_at(y, r, c) || 4 * c >= hd) continue;
+    const uint32_t i = run.i0 + r / G, g = h * G + r % G;
+    if (STEP) qv[y] = four_of(a.q + (size_t)i * a.q_stride + g * hd + 4 * c, a.nsl, a.sl_stride);
+    else qv[y] = *reinterpret_cast<const float4*>(a.qr + ((size_t)i * a.n_heads + g) * hd + 4 * c);
+  }
+  BlockRows<NS> ob;
+  const uint32_t block = run.pos0 / kKv8Block, r0 = run.pos0 % kKv8Block;
+  if (mine) {
+    if (STEP) {
+      if (e.fresh && h == 0 && t == 0) e.pages[run.pos0 / p.bs] = e.page;  // for the calls after this one
+      ob.load(a, run.table, r0, 1, h, [&](uint32_t) { return x; });
+    } else {
+      const float* src = a.own + ((size_t)run.job * 2 * p.n_kv + h) * kKv8Block * hd;
+#pragma unroll
+      for (uint32_t y = 0; y < NS; y++) {
+        const uint32_t i = t + 256 * y;
+        ob.v[y] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (4 * ob.col(i) < hd)
+          ob.v[y] = *reinterpret_cast<const float4*>(src + (size_t)ob.value(i) * p.n_kv * kKv8Block * hd + ob.row(i) * hd + 4 * ob.col(i));
+      }
     }
-    reinterpret_cast<float2*>(qs + r * QS)[c] = w;
+  }
+#pragma unroll
+  for (int y = 0; y < QN; y++) {
+    uint32_t r, c;
+    if (!q_at(y, r, c)) continue;
+    if (STEP && 4 * c < hd) qv[y] = turned(p, qv[y], c, run.pos0);
+    *reinterpret_cast<float4*>(qs + r * QS + 4 * c) = qv[y];
   }
   if (mine) {
     if (STEP) {
-      const uint32_t block = run.pos0 / kKv8Block, r0 = run.pos0 % kKv8Block;
-      if (e.fresh && h == 0 && t == 0) e.pages[run.pos0 / p.bs] = e.page;  // for the calls after this one
-      block_rows(a, run.table, block, r0, 1, h, kt, vt, hs, [&](uint32_t) { return x; });
-      __syncthreads();
-      if (r0 == kKv8Block - 1) hold_block(p, kv8_block(p, e.page, block, h), kt, vt, hs, block_max(kt, vt, hd, hs, red));
-      put_open(p, run.table, r0 + 1, h, kt, vt, hs);
-    } else {
-      const float* src = a.own + ((size_t)run.job * 2 * p.n_kv + h) * kKv8Block * hd;
-      for (uint32_t y = t; y < kKv8Block * hd; y += 256) {
-        kt[y / hd * hs + y % hd] = src[y];
-        vt[y / hd * hs + y % hd] = src[(size_t)p.n_kv * kKv8Block * hd + y];
-      }
+      ob.turn_keys(p, block, r0, 1);
+      ob.put_global(p, p.open + (size_t)run.table * 2 * p.n_kv * kKv8Block * hd, h, r0 + 1);
+    }
+    ob.put(kt, vt, hs);
+    if (STEP && r0 == kKv8Block - 1) {
+      const uint2 m = ob.largest(red);  // with a barrier
+      hold_block<NS>(p, kv8_block(p, e.page, block, h), kt, vt, hs, m);
     }
   }
   __syncthreads();
@@ -537,7 +676,8 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
           s[q] = mfma16(kf, qh[c], s[q]);
         }
       }
-      const float ck = sk * cq, svn0 = sv;
+      const float ck = sk * cq;
+      float svn = sv;
       const uint32_t k0 = kb + kKv8Block * kg;
       const bool edge = kb < start_max || kb + 64 > hi;  // the same in every lane
       kb += 256;
@@ -546,11 +686,6 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
         find(kb);
         load_k();
       }
-      float svn = svn0;
-#pragma unroll
-      for (int q = 0; q < 4; q++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) s[q][r] *= ck;
       if (edge) {
 #pragma unroll
         for (int q = 0; q < 4; q++)
@@ -559,19 +694,21 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
             const uint32_t pk = k0 + 4 * q + r;
             if (pk < start_n || pk >= hi) s[q][r] = -INFINITY;
           }
-        if (k0 >= hi || k0 + kKv8Block <= start_n) svn = 0.0f;  // no position of the block is attended to
+        if (k0 >= hi || k0 + kKv8Block <= start_n) {  // no position of the block is attended to
+          svn = 0.0f;
+        }
       }
+      // scores are s ck (a block's scale is a lane's, and not negative: the largest s is the largest score),
+      // weights 2^(s ck - M), at most 2^14: M is the largest score less 14. A NaN or +inf score
+      // makes L a NaN.
       float mt = -INFINITY;
 #pragma unroll
       for (int q = 0; q < 4; q++)
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          bad |= __builtin_amdgcn_classf(s[q][r], 0x203);  // NaN or +inf
-          mt = fmaxf(mt, s[q][r]);
-        }
-      mt = fmaxf(M, max16_32(mt) - 14.0f);
+        for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[q][r]);
+      const bool none = mt == -INFINITY;  // as 0 times it is a NaN
+      mt = fmaxf(M, max16_32(none ? mt : mt * ck) - 14.0f);
       const int en = max(ev, (int)max16_32((float)pow2_of(svn)));
-      // weights are 2^(s - M), at most 2^14: M is the largest score less 14
       const float mu = mt == -INFINITY ? 0.0f : mt;
       float f = __builtin_amdgcn_exp2f(M - mu);
       L *= f;
@@ -593,7 +730,9 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
         for (int q = 0; q < 2; q++)
 #pragma unroll
           for (int r = 0; r < 4; r++) {
-            const float pv = __builtin_amdgcn_exp2f(s[2 * y + q][r] - mu);
+            const float sv1 = s[2 * y + q][r];
+            float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(sv1, ck, -mu));
+            if (edge && sv1 == -INFINITY) pv = 0.0f;
             L += pv;
             w[4 * q + r] = pv * vn;
           }
@@ -613,7 +752,7 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
     }
   // the waves' sums joined through LDS, the values' in natural units
   L = sum16_32(L);
-  bad = max16_32(bad ? 1.0f : 0.0f) != 0.0f;
+  bad |= L != L || M == INFINITY;
   const float fo = pow2(ev);
   if (n16 < rows) {
     if (kg == 0) {
@@ -693,9 +832,10 @@ __global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
   }
   if (r >= run.n * G) return;
   const size_t rows = (size_t)part.nx * part.n_kv * part.R, row = part.row(0, x, h, r);
+  const uint32_t nparts = STEP ? kv8_parts_of(run.pos0, a.window && run.pos0 + 1 > a.window ? run.pos0 + 1 - a.window : 0) : a.nparts;
   float m = -INFINITY;
   bool bad = false;
-  for (uint32_t s = t; s < a.nparts; s += 256) {
+  for (uint32_t s = t; s < nparts; s += 256) {
     const float v = part.ml[s * rows + row].x;
     bad |= v != v;
     m = fmaxf(m, v);
@@ -709,14 +849,14 @@ __global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
   float l = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   if (g < ng && !uniform)
-    for (uint32_t s0 = g; s0 < a.nparts; s0 += 4 * ng) {
+    for (uint32_t s0 = g; s0 < nparts; s0 += 4 * ng) {
       float2 v[4];
       float4 w[4];
 #pragma unroll
       for (uint32_t k = 0; k < 4; k++) {
         const uint32_t s = s0 + k * ng;
         v[k] = make_float2(-INFINITY, 0.0f);
-        if (s < a.nparts) {
+        if (s < nparts) {
           v[k] = part.ml[s * rows + row];
           w[k] = reinterpret_cast<const float4*>(part.o + (s * rows + row) * hd)[c];
         }
@@ -906,15 +1046,19 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   int ev = -100;
   // a lane's key of the MFMA's row l32: 8 consecutive ones of a block to a half
   const uint32_t arow = 16 * (l32 / 16) + 8 * (l32 / 4 % 2) + 4 * (l32 / 8 % 2) + l32 % 4;
-  // scores s (scaled, masked), each eight of a block whose values have the scale svn, to weights and the row's sums
-  auto soften = [&](float* s, int n, const float* svn, float* w) {
+  // products s (masked), each eight of a block whose scores are s ck and whose values have the scale svn, to
+  // weights and the row's sums; as in k8_rows. edge: some product is masked.
+  auto soften = [&](const float* s, const int n, const float* ck, const float* svn, bool edge, float* w) {
     float mt = -INFINITY;
     int en = ev;
-    for (int y = 0; y < n; y++) {
-      odd |= __builtin_amdgcn_classf(s[y], 0x203);
-      mt = fmaxf(mt, s[y]);
+#pragma unroll
+    for (int y = 0; y < n / 8; y++) {
+      float mb = s[8 * y];
+#pragma unroll
+      for (int r = 1; r < 8; r++) mb = fmaxf(mb, s[8 * y + r]);
+      mt = fmaxf(mt, mb == -INFINITY ? mb : mb * ck[y]);
+      en = max(en, pow2_of(svn[y]));
     }
-    for (int y = 0; y < n / 8; y++) en = max(en, pow2_of(svn[y]));
     mt = fmaxf(M, max32(mt) - 14.0f);
     const float mu = mt == -INFINITY ? 0.0f : mt;
     float f = __builtin_amdgcn_exp2f(M - mu);
@@ -930,10 +1074,16 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     ev = en;
     const float un = pow2(-en);
     float sum = 0.0f;
-    for (int y = 0; y < n; y++) {
-      const float pv = __builtin_amdgcn_exp2f(s[y] - mu);
-      sum += pv;
-      w[y] = pv * (svn[y / 8] * un);
+#pragma unroll
+    for (int y = 0; y < n / 8; y++) {
+      const float vn = svn[y] * un;
+#pragma unroll
+      for (int r = 0; r < 8; r++) {
+        float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + r], ck[y], -mu));
+        if (edge && s[8 * y + r] == -INFINITY) pv = 0.0f;
+        sum += pv;
+        w[8 * y + r] = pv * vn;
+      }
     }
     L += sum;
   };
@@ -948,7 +1098,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     }
     if (busy && kb < w_hi && kb + 64 > w_lo) {
       const uint8_t* kbuf = lds + buf * BUF;
-      float s[32], w[32], svn[4];
+      float s[32], w[32], svn[4], ck[4];
 #pragma unroll
       for (uint32_t b = 0; b < 2; b++) {
         f32x16 acc = zero;
@@ -963,12 +1113,13 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         for (uint32_t y = 0; y < 2; y++) {
           const float2 c = sc[buf][2 * b + y];
           svn[2 * b + y] = c.y;
-          const float ck = c.x * cq;
-#pragma unroll
-          for (uint32_t r = 0; r < 8; r++) s[16 * b + 8 * y + r] = acc[8 * y + r] * ck;
+          ck[2 * b + y] = c.x * cq;
         }
+#pragma unroll
+        for (uint32_t r = 0; r < 16; r++) s[16 * b + r] = acc[r];
       }
-      if (kb < w_in0 || kb + 64 > w_in1) {  // positions that some row of the wave does not attend to
+      const bool edge = kb < w_in0 || kb + 64 > w_in1;  // positions that some row of the wave does not attend to
+      if (edge) {
         const uint32_t top = min(own, hi);
 #pragma unroll
         for (uint32_t y = 0; y < 4; y++) {
@@ -981,7 +1132,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
           }
         }
       }
-      soften(s, 32, svn, w);
+      soften(s, 32, ck, svn, edge, w);
 #pragma unroll
       for (uint32_t y = 0; y < 4; y++) {
         f16x8 wh, wl;
@@ -1028,15 +1179,11 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         const float u = key < 16 ? up[0].x : up[1].x;
         const float f[4] = {v.x * u, v.y * u, v.z * u, v.w * u};
         uint8_t* dst = lds + key * HDP * 2 + (((d / 8) ^ (key % KX)) * 16 + 8 * (d / 4 % 2));
-        f16x2 hi2[2], lo2[2];
+        uint32_t hi2[2], lo2[2];
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
-          hi2[y] = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(f[2 * y], f[2 * y + 1]));
-          lo2[y][0] = (_Float16)(f[2 * y] - (float)hi2[y][0]);
-          lo2[y][1] = (_Float16)(f[2 * y + 1] - (float)hi2[y][1]);
-        }
-        *reinterpret_cast<u32x2*>(dst) = u32x2{__builtin_bit_cast(uint32_t, hi2[0]), __builtin_bit_cast(uint32_t, hi2[1])};
-        *reinterpret_cast<u32x2*>(dst + PK) = u32x2{__builtin_bit_cast(uint32_t, lo2[0]), __builtin_bit_cast(uint32_t, lo2[1])};
+        for (int y = 0; y < 2; y++) split2(f[2 * y], f[2 * y + 1], hi2[y], lo2[y]);
+        *reinterpret_cast<u32x2*>(dst) = u32x2{hi2[0], hi2[1]};
+        *reinterpret_cast<u32x2*>(dst + PK) = u32x2{lo2[0], lo2[1]};
       }
       for (uint32_t it = t; it < 16 * (HDP / 4); it += 512) {
         const uint32_t kp = it % 16, d = it / 16 * 4, key = 2 * kp;
@@ -1050,11 +1197,11 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         const float f[4][2] = {{v0.x * u, v1.x * u}, {v0.y * u, v1.y * u}, {v0.z * u, v1.z * u}, {v0.w * u, v1.w * u}};
 #pragma unroll
         for (uint32_t y = 0; y < 4; y++) {
-          const f16x2 hi2 = __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(f[y][0], f[y][1]));
-          const f16x2 lo2 = {(_Float16)(f[y][0] - (float)hi2[0]), (_Float16)(f[y][1] - (float)hi2[1])};
+          uint32_t hi2, lo2;
+          split2(f[y][0], f[y][1], hi2, lo2);
           uint8_t* dst = lds + 2 * PK + (d + y) * 64 + (((key / 8) ^ ((d + y) / 2 % 4)) * 16 + 2 * (key % 8));
-          *reinterpret_cast<uint32_t*>(dst) = __builtin_bit_cast(uint32_t, hi2);
-          *reinterpret_cast<uint32_t*>(dst + PV) = __builtin_bit_cast(uint32_t, lo2);
+          *reinterpret_cast<uint32_t*>(dst) = hi2;
+          *reinterpret_cast<uint32_t*>(dst + PV) = lo2;
         }
       }
       __syncthreads();
@@ -1069,20 +1216,20 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
           acc = mfma32(kh, ql[st], acc);
           acc = mfma32(kh, qh[st], acc);
         }
-        float s[16], w[16], sn[2];
+        float s[16], w[16], sn[2], ck[2];
 #pragma unroll
         for (uint32_t y = 0; y < 2; y++) {
           const bool at = own == k0 + 16 * y;
           odd |= at && wild[y];
           sn[y] = at && !wild[y] ? svn[y] : 0.0f;
-          const float ck = skn[y] * cq;
+          ck[y] = skn[y] * cq;
 #pragma unroll
           for (uint32_t r = 0; r < 8; r++) {
             const uint32_t pk = k0 + 16 * y + 8 * hf + r;
-            s[8 * y + r] = at && !wild[y] && pk <= pos && pk >= start ? acc[8 * y + r] * ck : -INFINITY;
+            s[8 * y + r] = at && !wild[y] && pk <= pos && pk >= start ? acc[8 * y + r] : -INFINITY;
           }
         }
-        soften(s, 16, sn, w);
+        soften(s, 16, ck, sn, true, w);
 #pragma unroll
         for (uint32_t y = 0; y < 2; y++) {
           f16x8 wh, wl;
@@ -1104,7 +1251,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     const LanePair l = xor32_pair(L);
     L = l.a + l.b;
   }
-  odd = max32(odd ? 1.0f : 0.0f) != 0.0f;
+  odd = max32(odd ? 1.0f : 0.0f) != 0.0f || L != L || M == INFINITY;
   const float fo = pow2(ev);
   if (mine) {
     if (hf == 0) part.ml[prow] = make_float2(odd ? __uint_as_float(kBadRow) : M, L);
@@ -1255,28 +1402,53 @@ __global__ void __launch_bounds__(256) k8_join_tile(Kv8Args a) {
 }
 
 // grid (chunks, n_kv), 256 threads: rows of one block, from its codes or from the open rows.
+template <int NS>
 __global__ void __launch_bounds__(256) k8_read(Kv8Pool p, const Kv8Rows* rows, Kv8RowsInline inl, float* k, float* v) {
+  constexpr uint32_t HDP = 32 * NS, Q4 = HDP / 4;
+  __shared__ uint32_t vt[kKv8Block * HDP / 4];
   const Kv8Rows r = rows ? rows[blockIdx.x] : inl.r[blockIdx.x];
-  const uint32_t h = blockIdx.y, hd = p.hd, kvd = p.n_kv * hd;
-  float* dk = k + (size_t)r.i0 * kvd + h * hd;
-  float* dv = v + (size_t)r.i0 * kvd + h * hd;
+  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, kvd = p.n_kv * hd;
+  auto put = [&](float* to, uint32_t row, uint32_t c, float4 w) {  // the caller's rows: any float's alignment
+    *reinterpret_cast<f32x4u*>(to + (size_t)(r.i0 + row) * kvd + h * hd + 4 * c) = f32x4u{w.x, w.y, w.z, w.w};
+  };
   if (!r.whole) {
-    const float* src = kv8_open(p, r.table, h) + r.r0 * hd;
-    for (uint32_t x = threadIdx.x; x < r.n * hd; x += 256) {
-      const size_t to = (size_t)(x / hd) * kvd + x % hd;
-      dk[to] = src[x];
-      dv[to] = src[(size_t)p.n_kv * kKv8Block * hd + x];
+    const float* src = kv8_open(p, r.table, h);
+#pragma unroll
+    for (uint32_t y = 0; y < NS; y++) {
+      const uint32_t i = t + 256 * y, val = i / (16 * Q4), row = i / Q4 % 16, c = i % Q4;
+      if (row < r.n && 4 * c < hd)
+        put(val ? v : k, row, c, *reinterpret_cast<const float4*>(src + (size_t)val * p.n_kv * kKv8Block * hd + (r.r0 + row) * hd + 4 * c));
     }
     return;
   }
   const size_t u = kv8_block(p, kv8_page(p, r.table, r.block), r.block, h);
-  const uint8_t* c = kv8_codes(p, u);
-  const float sk = p.scales[2 * u], sv = p.scales[2 * u + 1];
-  for (uint32_t x = threadIdx.x; x < r.n * hd; x += 256) {
-    const uint32_t row = r.r0 + x / hd, d = x % hd;
-    const size_t to = (size_t)(x / hd) * kvd + d;
-    dk[to] = (float)((int)c[kv8_key(p.hdp, row, d)] - 128) * sk;
-    dv[to] = (float)((int)c[kKv8Block * p.hdp + d * kKv8Block + row] - 128) * sv;
+  const uint8_t* codes = kv8_codes(p, u);
+  const float2 sc = reinterpret_cast<const float2*>(p.scales)[u];
+  auto value = [](uint32_t w, uint32_t b, float s) { return (float)((int)(w >> 8 * b & 255u) - 128) * s; };
+  const uint32_t* vw = reinterpret_cast<const uint32_t*>(codes + kKv8Block * HDP);
+  constexpr uint32_t W = kKv8Block * HDP / 4;
+#pragma unroll
+  for (uint32_t y = 0; y < W; y += 256) {
+    const uint32_t i = t + y, row = i / Q4, c = i % Q4;
+    if (W % 256 && i >= W) break;
+    vt[i] = vw[i];  // word d * 4 + row / 4
+    if (row < r.n && 4 * c < hd) {
+      const uint32_t w = *reinterpret_cast<const uint32_t*>(codes + kv8_key(HDP, r.r0 + row, 4 * c));
+      put(k, row, c, make_float4(value(w, 0, sc.x), value(w, 1, sc.x), value(w, 2, sc.x), value(w, 3, sc.x)));
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (uint32_t y = 0; y < W; y += 256) {
+    const uint32_t i = t + y, row = i / Q4, c = i % Q4;
+    if (W % 256 && i >= W) break;
+    if (row < r.n && 4 * c < hd) {
+      const uint32_t a = r.r0 + row;
+      float f[4];
+#pragma unroll
+      for (uint32_t d = 0; d < 4; d++) f[d] = value(vt[(4 * c + d) * 4 + a / 4], a % 4, sc.y);
+      put(v, row, c, make_float4(f[0], f[1], f[2], f[3]));
+    }
   }
 }
 
@@ -1313,30 +1485,36 @@ template <int NS, bool STEP>
 void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
   // what 16 rows of the widest heads of this build take, set once; a call asks for its own rows'
   static const bool set = [] {
-    const int most = (int)kv8_rows_lds(32 * NS, 32 * NS, 16);
+    const int most = (int)kv8_rows_lds(32 * NS, 16);
     return hipFuncSetAttribute((const void*)k8_rows<NS, STEP, true>, hipFuncAttributeMaxDynamicSharedMemorySize, most) == hipSuccess &&
            hipFuncSetAttribute((const void*)k8_rows<NS, STEP, false>, hipFuncAttributeMaxDynamicSharedMemorySize, most) == hipSuccess;
   }();
   (void)set;
   const bool one = one_part(a, STEP);
   const uint32_t G = a.n_heads / a.p.n_kv, rows = STEP ? G : kv8_group_tokens(G) * G, nx = STEP ? a.n : a.nrun;
-  const uint32_t lds = kv8_rows_lds(a.p.hd, a.p.hdp, rows);
-  const dim3 grid(nx, a.p.n_kv, one ? 1 : a.nparts);
+  const uint32_t lds = kv8_rows_lds(a.p.hdp, rows);
+  const dim3 grid = one ? dim3(nx, a.p.n_kv) : STEP ? dim3(a.items, a.p.n_kv) : dim3(nx, a.p.n_kv, a.nparts);
   auto kernel = one ? k8_rows<NS, STEP, true> : k8_rows<NS, STEP, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, inl);
   if (!one) hipLaunchKernelGGL(k8_join<STEP>, dim3(nx, a.p.n_kv * rows), dim3(256), 0, st, a, inl);
 }
 
+// f of the build for the heads' width
+template <class F>
+void by_width(uint32_t hdp, F&& f) {
+  switch (hdp / 32) {
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 3: f(std::integral_constant<int, 3>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 6: f(std::integral_constant<int, 6>()); break;
+    default: f(std::integral_constant<int, 8>()); break;
+  }
+}
+
 template <bool STEP>
 hipError_t launch_rows_of(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
-  switch (a.p.hdp / 32) {
-    case 1: launch_rows<1, STEP>(a, inl, st); break;
-    case 2: launch_rows<2, STEP>(a, inl, st); break;
-    case 3: launch_rows<3, STEP>(a, inl, st); break;
-    case 4: launch_rows<4, STEP>(a, inl, st); break;
-    case 6: launch_rows<6, STEP>(a, inl, st); break;
-    default: launch_rows<8, STEP>(a, inl, st); break;
-  }
+  by_width(a.p.hdp, [&](auto ns) { launch_rows<ns(), STEP>(a, inl, st); });
   return hipGetLastError();
 }
 
@@ -1345,8 +1523,8 @@ hipError_t launch_rows_of(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) { return launch_rows_of<true>(a, inl, st); }
 
 hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
-  const uint32_t lds = 2 * kKv8Block * a.p.hd * 4 + (a.qr ? kKv8Block * a.p.hd / 2 * 16 : 0);
-  hipLaunchKernelGGL(k8_append, dim3(a.njob, a.p.n_kv), dim3(256), lds, st, a);
+  const dim3 jobs(a.njob, a.p.n_kv, a.qr ? 1 + (a.n_heads / a.p.n_kv + 3) / 4 : 1);
+  by_width(a.p.hdp, [&](auto ns) { hipLaunchKernelGGL(k8_append<ns()>, jobs, dim3(256), 0, st, a); });
   if (!a.ctx) return hipGetLastError();
   if (a.ntile) {
     const dim3 grid(a.p.n_kv, a.ntile, a.tsplits);
@@ -1364,7 +1542,9 @@ hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
 
 hipError_t launch_kv8_read(const Kv8Pool& p, const Kv8Rows* rows, const Kv8RowsInline& inl, uint32_t nrows, float* k,
                            float* v, hipStream_t st) {
-  hipLaunchKernelGGL(k8_read, dim3(nrows, p.n_kv), dim3(256), 0, st, p, rows, inl, k, v);
+  by_width(p.hdp, [&](auto ns) {
+    hipLaunchKernelGGL(k8_read<ns()>, dim3(nrows, p.n_kv), dim3(256), 0, st, p, rows, inl, k, v);
+  });
   return hipGetLastError();
 }
 

@@ -512,6 +512,9 @@ struct Kv8Rows {
 // one is the row's own block; the others begin at a block's start).
 constexpr uint32_t kKv8Split = 512;
 constexpr uint32_t kv8_parts(uint32_t span) { return 1 + (span + kKv8Block - 1 + kKv8Split - 1) / kKv8Split; }
+constexpr uint32_t kv8_parts_of(uint32_t pos, uint32_t start) {  // of an entry
+  return 1 + (pos / kKv8Block * kKv8Block - start / kKv8Block * kKv8Block + kKv8Split - 1) / kKv8Split;
+}
 constexpr uint32_t kv8_group_tokens(uint32_t heads) { return 16 / heads; }  // of 16 rows
 constexpr uint32_t kKv8TileRows = 256, kKv8TileHd = 128;  // and the widest heads that tiles take
 constexpr uint32_t kv8_tile_tokens(uint32_t heads) { return kKv8TileRows / heads; }
@@ -535,6 +538,7 @@ struct Kv8Args {
   float2* own_max;     //   and [njob][n_kv] their largest magnitudes (keys, values)
   float* part;         // partial sums of the groups' rows (kv8_part_floats): the own block,
   uint32_t nparts;     //   then as many splits as the longest span has
+  uint32_t items;      // a step's parts, over all entries
   float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions
   uint32_t tsplits, tkeys;
 };

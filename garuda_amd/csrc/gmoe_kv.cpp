@@ -431,6 +431,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     Kv8Inline inl{};
     const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
     a.nparts = kv8_parts(maxspan);
+    for (uint32_t i = 0; i < n; i++) a.items += kv8_parts_of(ent[i].pos, ent[i].start);
     if (gmoe_status s = grow_scratch(kv, eb + step8_bytes(kv, n, a.nparts))) return s;
     if (eb)
       if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
@@ -861,6 +862,7 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
     a.sl_stride = sl_stride;
     a.part = reinterpret_cast<float*>(kv->scratch);
     a.nparts = kv8_parts(nchunk * kAttnChunk);
+    a.items = n * a.nparts;
     if (step_bytes(kv, n, nchunk) > kv->scratch_bytes) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
     KV_TRY(launch_kv8_step(a, Kv8Inline{}, st));
     return GMOE_OK;
