@@ -124,7 +124,7 @@ SIGNATURES = {
     "gmoe_kv_free_pages": (i32, [vp, C.POINTER(u64)]),
     "gmoe_kv_fail_reserves": (i32, [vp, u32]),
     "gmoe_attention": (i32, [vp, u32, u32p, u32, f32p, f32p, f32p, f32p]),
-    "gmoe_attention_async": (i32, [vp, u32, u32p, u32, vp, vp, vp, vp, vp]),
+    "gmoe_attention_async": (i32, [vp, u32, vp, u32, vp, vp, vp, vp, vp]),
     "gmoe_gguf_open": (i32, [C.c_char_p, C.POINTER(vp)]),
     "gmoe_gguf_parse": (i32, [vp, u64, C.POINTER(vp)]),
     "gmoe_gguf_close": (None, [vp]),

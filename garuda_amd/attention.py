@@ -30,6 +30,8 @@ class GmoeKvDesc(C.Structure):
 
 
 def _u32(a) -> np.ndarray:
+    if type(a) is np.ndarray and a.dtype == np.uint32 and a.ndim == 1 and a.flags.c_contiguous:
+        return a
     return np.ascontiguousarray(np.asarray(a, dtype=np.uint32).reshape(-1))
 
 
@@ -86,9 +88,9 @@ class KvCache:
         return out
 
     def attention_async(self, layer: int, seqs, d_q: int, d_k: int, d_v: int, d_out: int, stream: int = 0) -> None:
-        seqs = np.ascontiguousarray(np.asarray(seqs, dtype=np.uint32).reshape(-1))
-        _check(lib().gmoe_attention_async(self._h, layer, seqs.ctypes.data_as(C.POINTER(C.c_uint32)), seqs.size,
-                                          d_q or None, d_k or None, d_v or None, d_out or None, stream or None))
+        seqs = _u32(seqs)
+        _check(lib().gmoe_attention_async(self._h, layer, seqs.ctypes.data, seqs.size, d_q or None, d_k or None,
+                                          d_v or None, d_out or None, stream or None))
 
     def append(self, layer: int, seqs, k: np.ndarray, v: np.ndarray) -> None:
         """One token per entry, as `attention` takes them, without queries."""

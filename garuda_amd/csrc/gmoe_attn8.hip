@@ -192,7 +192,7 @@ __device__ __forceinline__ void hold_block(const Kv8Pool& p, size_t unit, const 
   }
 }
 
-// grid (njob, n_kv, 1 + ceil(G / 4) where the call attends), 256 threads: a block of the call's
+// grid (njob * n_kv, 1, 1 + ceil(G / 4) where the call attends), 256 threads: a block of the call's
 // positions and one kv head's keys and values (z 0), or up to four of its query heads, whose
 // turned rows go to a.qr. The job of a sequence's first block writes the open rows of its last
 // one, after it has read those that were there. Copies the call's groups and tiles to the
@@ -204,12 +204,12 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
   __shared__ uint32_t red[8];
   __shared__ Kv8Job job;
   const Kv8Pool& p = a.p;
-  const uint32_t h = blockIdx.y, t = threadIdx.x;
+  const uint32_t h = blockIdx.x % p.n_kv, jb = blockIdx.x / p.n_kv, t = threadIdx.x;
   auto take = [&](uint32_t i) {  // job i, from pinned memory
     if (t < sizeof(Kv8Job) / 4) reinterpret_cast<uint32_t*>(&job)[t] = reinterpret_cast<const uint32_t*>(a.hjob + i)[t];
     __syncthreads();
   };
-  take(blockIdx.x);
+  take(jb);
   if (blockIdx.z) {
     const uint32_t G = a.n_heads / p.n_kv, g0 = 4 * (blockIdx.z - 1), ng = min(G - g0, 4u);
     float4 q[2 * NS];  // float4 t + 256 y of [ng][16][HDP], in flight together
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
   if (h == 0 && t == 0 && (flags & kKv8Fresh))
     p.tables[(size_t)job.table * p.ppseq + job.block / (p.bs / kKv8Block)] = job.page;
   if (h == 0 && a.qr)
-    for (uint32_t x = blockIdx.x * 256 + t; x < a.nrun + a.ntile; x += gridDim.x * 256) a.run[x] = a.hrun[x];
+    for (uint32_t x = jb * 256 + t; x < a.nrun + a.ntile; x += a.njob * 256) a.run[x] = a.hrun[x];
   BlockRows<NS> rows;
   auto get = [&] {
     rows.load(a, job.table, job.r0, job.n, h, [&](uint32_t r) { return job.ent[r]; });
@@ -249,8 +249,8 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
   if (a.qr || (flags & kKv8Whole)) {
     const uint2 m = rows.largest(red);
     if (a.qr) {
-      rows.put_global(p, a.own + (size_t)blockIdx.x * 2 * p.n_kv * kKv8Block * p.hd, h, kKv8Block);
-      if (t == 0) a.own_max[(size_t)blockIdx.x * p.n_kv + h] = make_float2(__uint_as_float(m.x), __uint_as_float(m.y));
+      rows.put_global(p, a.own + (size_t)jb * 2 * p.n_kv * kKv8Block * p.hd, h, kKv8Block);
+      if (t == 0) a.own_max[(size_t)jb * p.n_kv + h] = make_float2(__uint_as_float(m.x), __uint_as_float(m.y));
     }
     if (flags & kKv8Whole) {
       rows.put(kt, vt, HS);
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
     }
   }
   if (!(flags & kKv8First)) return;
-  if (last != blockIdx.x) {
+  if (last != jb) {
     __syncthreads();
     take(last);
     get();
@@ -347,6 +347,9 @@ __device__ __forceinline__ int pow2_of(float x) {
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
 
+// A score's scale where the block's is 0, as its products are: for masked ones, -inf, to stay that.
+__device__ __forceinline__ float above0(float x) { return x == 0.0f ? 1.0f : x; }
+
 constexpr float kLog2e = 0x1.715476p+0f;
 constexpr uint32_t kBadRow = 0x7fc00000u;  // a part's maximum: a NaN or +inf score
 
@@ -429,7 +432,9 @@ __device__ __forceinline__ bool step_part(const Kv8Args& a, const Kv8Inline& inl
 
 // STEP: groups are entries, and the token is appended here. ONE: one workgroup takes both
 // the own block and what is before it (at most kKv8Split positions), and writes the context.
-// grid: (groups, n_kv, parts), in a step without ONE (parts of all entries, n_kv).
+// grid: (groups * n_kv, 1, parts), in a step without ONE (parts of all entries * n_kv). The kv
+// head runs fastest: a page's heads follow each other, and workgroups of one head alone would
+// read an eighth of the memory's channels at a time (8 sequences at 65000: 228 us that way).
 template <int NS, bool STEP, bool ONE>
 __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8Inline inl) {
   constexpr uint32_t HDP = 32 * NS, NP = NS / 2, QS = kv8_pad(HDP), Q4 = HDP / 4;
@@ -437,15 +442,15 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   __shared__ uint32_t red[8];
   __shared__ float own_m[16], own_l[16], wm[4][16], wl[4][16];
   const Kv8Pool& p = a.p;
-  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
+  const uint32_t h = blockIdx.x % p.n_kv, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
   const uint32_t lane = t & 63, n16 = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  uint32_t x = blockIdx.x, z = blockIdx.z;
+  uint32_t x = blockIdx.x / p.n_kv, z = blockIdx.z;
   Kv8Run run;
   AttnEntry e{};
   if (STEP) {
     if (ONE) e = a.ent ? a.ent[x] : inl.e[x];
-    else if (!step_part(a, inl, blockIdx.x, x, z, e)) return;
+    else if (!step_part(a, inl, x, x, z, e)) return;
     run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
   } else {
     run = a.run[x];
@@ -935,6 +940,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   constexpr uint32_t KX = CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;             // keys' column x is at x ^ (key % KX)
   constexpr uint32_t KB = 64 * HDP * 2, BUF = 2 * KB;                          // bytes of a tile's keys; of a buffer
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
+  __shared__ u32x4 qlo[8 * KS * 64];  // the queries' second halves: in registers they would spill
   __shared__ float2 sc[2][4];
   const Kv8Pool& p = a.p;
   const uint32_t h = blockIdx.x, x = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
@@ -1004,7 +1010,9 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     unit = find(lo + 64);
   }
   // queries: the wave's B operand
-  f16x8 qh[KS], ql[KS];
+  f16x8 qh[KS];
+  u32x4* qlw = qlo + wave * KS * 64 + lane;
+  auto ql = [&](uint32_t st) { return __builtin_bit_cast(f16x8, qlw[64 * st]); };
   float cq;
   bool odd;
   {
@@ -1034,58 +1042,125 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
                     v[s][1].x * up, v[s][1].y * up, v[s][1].z * up, v[s][1].w * up};
       if (odd)
         for (int y = 0; y < 8; y++) f[y] = 0.0f;
-      split8(f, qh[s], ql[s]);
+      f16x8 lo8;
+      split8(f, qh[s], lo8);
+      qlw[64 * s] = __builtin_bit_cast(u32x4, lo8);  // a lane's own
     }
   }
-  f32x16 o[NS], zero;
+  f32x16 o[NS];
 #pragma unroll
-  for (int r = 0; r < 16; r++) zero[r] = 0.0f;
-#pragma unroll
-  for (int d = 0; d < NS; d++) o[d] = zero;
+  for (int d = 0; d < NS; d++) o[d] = (f32x16)(0.0f);
   float M = -INFINITY, L = 0.0f;
   int ev = -100;
   // a lane's key of the MFMA's row l32: 8 consecutive ones of a block to a half
   const uint32_t arow = 16 * (l32 / 16) + 8 * (l32 / 4 % 2) + 4 * (l32 / 8 % 2) + l32 % 4;
-  // products s (masked), each eight of a block whose scores are s ck and whose values have the scale svn, to
-  // weights and the row's sums; as in k8_rows. edge: some product is masked.
-  auto soften = [&](const float* s, const int n, const float* ck, const float* svn, bool edge, float* w) {
+  // Products s, each eight of a block whose scores are s ck and whose values have the scale svn, to
+  // weights and the row's sums. Weights are 2^(score - M): M is 8 below the largest score when
+  // it is set, and set again only where a score is more than 13 above it, as the sums' values'
+  // unit 2^ev is only where a scale is 4 times it or more. So few tiles rescale the sums (with
+  // M the running maximum, a tile of a long span in two did), weights times scales stay
+  // below 2^15, and what is left of them after the first fp16 has 11 bits down to 2^-11 of the
+  // largest weight, then to 2^-33 of it. A NaN or +inf score makes L a NaN. Masked products are
+  // -inf (every ck is above 0).
+  auto soften = [&](const float* s, const int n, const float* ck, const float* svn, int en, float* w) {
     float mt = -INFINITY;
-    int en = ev;
 #pragma unroll
     for (int y = 0; y < n / 8; y++) {
       float mb = s[8 * y];
 #pragma unroll
       for (int r = 1; r < 8; r++) mb = fmaxf(mb, s[8 * y + r]);
-      mt = fmaxf(mt, mb == -INFINITY ? mb : mb * ck[y]);
-      en = max(en, pow2_of(svn[y]));
+      mt = fmaxf(mt, mb * ck[y]);
     }
-    mt = fmaxf(M, max32(mt) - 14.0f);
-    const float mu = mt == -INFINITY ? 0.0f : mt;
-    float f = __builtin_amdgcn_exp2f(M - mu);
-    L *= f;
-    f *= pow2(max(ev - en, -126));
-    if (__ballot(f != 1.0f)) {
+    mt = max32(mt);
+    const bool up = mt - M > 13.0f;
+    if (__ballot(up) || en > ev + 1) {
+      asm volatile("");
+      const float mn = up ? mt - 8.0f : M, was = M;
+      M = mn;
+      float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(was - mn);
+      L *= f;
+      if (en > ev + 1) {
+        f *= pow2(max(ev - en, -126));
+        ev = en;
+      }
 #pragma unroll
       for (int d = 0; d < NS; d++)
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] *= f;
     }
-    M = mt;
-    ev = en;
-    const float un = pow2(-en);
+    const float mu = M == -INFINITY ? 0.0f : M, un = pow2(-ev);
     float sum = 0.0f;
 #pragma unroll
     for (int y = 0; y < n / 8; y++) {
       const float vn = svn[y] * un;
 #pragma unroll
       for (int r = 0; r < 8; r++) {
-        float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + r], ck[y], -mu));
-        if (edge && s[8 * y + r] == -INFINITY) pv = 0.0f;
+        const float pv = __builtin_amdgcn_exp2f(__builtin_fmaf(s[8 * y + r], ck[y], -mu));
         sum += pv;
         w[8 * y + r] = pv * vn;
       }
     }
     L += sum;
+  };
+  // 64 held positions from kb on, in a buffer
+  auto step = [&](uint32_t kb, uint32_t b) {
+    const uint8_t* kbuf = lds + b * BUF;
+    float s[32], w[32], svn[4], ck[4];
+    int en = -100;
+#pragma unroll
+    for (uint32_t y = 0; y < 4; y++) {
+      const uint32_t c = (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(sc[b][y].x));
+      const uint32_t v = (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(sc[b][y].y));
+      ck[y] = above0(__uint_as_float(c) * cq);
+      svn[y] = __uint_as_float(v);
+      en = max(en, pow2_of(__uint_as_float(v)));
+    }
+    f32x16 acc[2] = {(f32x16)(0.0f), (f32x16)(0.0f)};
+#pragma unroll
+    for (uint32_t st = 0; st < KS; st++) {
+      const f16x8 lo8 = ql(st);
+#pragma unroll
+      for (uint32_t y = 0; y < 2; y++) {
+        const uint32_t key = 32 * y + arow;
+        const f16x8 kf = *reinterpret_cast<const f16x8*>(kbuf + key * HDP * 2 + (((2 * st + hf) ^ (key % KX)) * 16));
+        acc[y] = mfma32(kf, lo8, acc[y]);
+        acc[y] = mfma32(kf, qh[st], acc[y]);
+      }
+    }
+#pragma unroll
+    for (uint32_t y = 0; y < 2; y++)
+#pragma unroll
+      for (uint32_t r = 0; r < 16; r++) s[16 * y + r] = acc[y][r];
+    if (kb < w_in0 || kb + 64 > w_in1) {  // some row of the wave does not attend to all
+      asm volatile("");                   // a branch: the selects of every tile were a fifth of its instructions
+      const uint32_t top = min(own, hi);
+#pragma unroll
+      for (uint32_t y = 0; y < 4; y++) {
+        const uint32_t k0 = kb + 16 * y;
+        if (k0 >= top || k0 + 16 <= start) {
+          svn[y] = 0.0f;
+          ck[y] = 1.0f;
+        }
+#pragma unroll
+        for (uint32_t r = 0; r < 8; r++) {
+          const uint32_t pk = k0 + 8 * hf + r;
+          if (pk < start || pk >= top) s[8 * y + r] = -INFINITY;
+        }
+      }
+    }
+    soften(s, 32, ck, svn, en, w);
+#pragma unroll
+    for (uint32_t y = 0; y < 4; y++) {
+      f16x8 wh, wl;
+      split8(w + 8 * y, wh, wl);
+#pragma unroll
+      for (uint32_t d = 0; d < NS; d++) {
+        const uint32_t dr = 32 * d + l32;
+        const f16x8 vf = *reinterpret_cast<const f16x8*>(kbuf + KB + dr * 128 + (((2 * y + hf) ^ (dr % 8)) * 16));
+        o[d] = mfma32(vf, wl, o[d]);
+        o[d] = mfma32(vf, wh, o[d]);
+      }
+    }
   };
   if (any) store(0);
   __syncthreads();
@@ -1097,54 +1172,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
       if (kb + 128 < hi) unit = find(kb + 128);
     }
     if (busy && kb < w_hi && kb + 64 > w_lo) {
-      const uint8_t* kbuf = lds + buf * BUF;
-      float s[32], w[32], svn[4], ck[4];
-#pragma unroll
-      for (uint32_t b = 0; b < 2; b++) {
-        f32x16 acc = zero;
-#pragma unroll
-        for (uint32_t st = 0; st < KS; st++) {
-          const uint32_t key = 32 * b + arow;
-          const f16x8 kf = *reinterpret_cast<const f16x8*>(kbuf + key * HDP * 2 + (((2 * st + hf) ^ (key % KX)) * 16));
-          acc = mfma32(kf, ql[st], acc);
-          acc = mfma32(kf, qh[st], acc);
-        }
-#pragma unroll
-        for (uint32_t y = 0; y < 2; y++) {
-          const float2 c = sc[buf][2 * b + y];
-          svn[2 * b + y] = c.y;
-          ck[2 * b + y] = c.x * cq;
-        }
-#pragma unroll
-        for (uint32_t r = 0; r < 16; r++) s[16 * b + r] = acc[r];
-      }
-      const bool edge = kb < w_in0 || kb + 64 > w_in1;  // positions that some row of the wave does not attend to
-      if (edge) {
-        const uint32_t top = min(own, hi);
-#pragma unroll
-        for (uint32_t y = 0; y < 4; y++) {
-          const uint32_t k0 = kb + 16 * y;
-          if (k0 >= top || k0 + 16 <= start) svn[y] = 0.0f;
-#pragma unroll
-          for (uint32_t r = 0; r < 8; r++) {
-            const uint32_t pk = k0 + 8 * hf + r;
-            if (pk < start || pk >= top) s[8 * y + r] = -INFINITY;
-          }
-        }
-      }
-      soften(s, 32, ck, svn, edge, w);
-#pragma unroll
-      for (uint32_t y = 0; y < 4; y++) {
-        f16x8 wh, wl;
-        split8(w + 8 * y, wh, wl);
-#pragma unroll
-        for (uint32_t d = 0; d < NS; d++) {
-          const uint32_t dr = 32 * d + l32;
-          const f16x8 vf = *reinterpret_cast<const f16x8*>(kbuf + KB + dr * 128 + (((2 * y + hf) ^ (dr % 8)) * 16));
-          o[d] = mfma32(vf, wl, o[d]);
-          o[d] = mfma32(vf, wh, o[d]);
-        }
-      }
+      step(kb, buf);
     }
     if (more) store(buf ^ 1);
     __syncthreads();
@@ -1207,13 +1235,13 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
       __syncthreads();
       const uint32_t k0 = b0 * kKv8Block;
       if (busy && k0 <= pw1 && k0 + 32 > own_of(pw0)) {
-        f32x16 acc = zero;
+        f32x16 acc = (f32x16)(0.0f);
 #pragma unroll
         for (uint32_t st = 0; st < KS; st++) {
           const uint8_t* at = lds + arow * HDP * 2 + (((2 * st + hf) ^ (arow % KX)) * 16);
           const f16x8 kh = *reinterpret_cast<const f16x8*>(at), kl = *reinterpret_cast<const f16x8*>(at + PK);
           acc = mfma32(kl, qh[st], acc);
-          acc = mfma32(kh, ql[st], acc);
+          acc = mfma32(kh, ql(st), acc);
           acc = mfma32(kh, qh[st], acc);
         }
         float s[16], w[16], sn[2], ck[2];
@@ -1222,14 +1250,14 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
           const bool at = own == k0 + 16 * y;
           odd |= at && wild[y];
           sn[y] = at && !wild[y] ? svn[y] : 0.0f;
-          ck[y] = skn[y] * cq;
+          ck[y] = above0(skn[y] * cq);
 #pragma unroll
           for (uint32_t r = 0; r < 8; r++) {
             const uint32_t pk = k0 + 16 * y + 8 * hf + r;
             s[8 * y + r] = at && !wild[y] && pk <= pos && pk >= start ? acc[8 * y + r] : -INFINITY;
           }
         }
-        soften(s, 16, ck, sn, true, w);
+        soften(s, 16, ck, sn, max(pow2_of(svn[0]), pow2_of(svn[1])), w);
 #pragma unroll
         for (uint32_t y = 0; y < 2; y++) {
           f16x8 wh, wl;
@@ -1401,13 +1429,13 @@ __global__ void __launch_bounds__(256) k8_join_tile(Kv8Args a) {
     }
 }
 
-// grid (chunks, n_kv), 256 threads: rows of one block, from its codes or from the open rows.
+// grid (chunks * n_kv), 256 threads: rows of one block, from its codes or from the open rows.
 template <int NS>
 __global__ void __launch_bounds__(256) k8_read(Kv8Pool p, const Kv8Rows* rows, Kv8RowsInline inl, float* k, float* v) {
   constexpr uint32_t HDP = 32 * NS, Q4 = HDP / 4;
   __shared__ uint32_t vt[kKv8Block * HDP / 4];
-  const Kv8Rows r = rows ? rows[blockIdx.x] : inl.r[blockIdx.x];
-  const uint32_t h = blockIdx.y, t = threadIdx.x, hd = p.hd, kvd = p.n_kv * hd;
+  const uint32_t h = blockIdx.x % p.n_kv, i0 = blockIdx.x / p.n_kv, t = threadIdx.x, hd = p.hd, kvd = p.n_kv * hd;
+  const Kv8Rows r = rows ? rows[i0] : inl.r[i0];
   auto put = [&](float* to, uint32_t row, uint32_t c, float4 w) {  // the caller's rows: any float's alignment
     *reinterpret_cast<f32x4u*>(to + (size_t)(r.i0 + row) * kvd + h * hd + 4 * c) = f32x4u{w.x, w.y, w.z, w.w};
   };
@@ -1493,7 +1521,7 @@ void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
   const bool one = one_part(a, STEP);
   const uint32_t G = a.n_heads / a.p.n_kv, rows = STEP ? G : kv8_group_tokens(G) * G, nx = STEP ? a.n : a.nrun;
   const uint32_t lds = kv8_rows_lds(a.p.hdp, rows);
-  const dim3 grid = one ? dim3(nx, a.p.n_kv) : STEP ? dim3(a.items, a.p.n_kv) : dim3(nx, a.p.n_kv, a.nparts);
+  const dim3 grid(a.p.n_kv * (STEP && !one ? a.items : nx), 1, STEP || one ? 1 : a.nparts);
   auto kernel = one ? k8_rows<NS, STEP, true> : k8_rows<NS, STEP, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, inl);
   if (!one) hipLaunchKernelGGL(k8_join<STEP>, dim3(nx, a.p.n_kv * rows), dim3(256), 0, st, a, inl);
@@ -1523,7 +1551,7 @@ hipError_t launch_rows_of(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) { return launch_rows_of<true>(a, inl, st); }
 
 hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
-  const dim3 jobs(a.njob, a.p.n_kv, a.qr ? 1 + (a.n_heads / a.p.n_kv + 3) / 4 : 1);
+  const dim3 jobs(a.njob * a.p.n_kv, 1, a.qr ? 1 + (a.n_heads / a.p.n_kv + 3) / 4 : 1);
   by_width(a.p.hdp, [&](auto ns) { hipLaunchKernelGGL(k8_append<ns()>, jobs, dim3(256), 0, st, a); });
   if (!a.ctx) return hipGetLastError();
   if (a.ntile) {
@@ -1543,7 +1571,7 @@ hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
 hipError_t launch_kv8_read(const Kv8Pool& p, const Kv8Rows* rows, const Kv8RowsInline& inl, uint32_t nrows, float* k,
                            float* v, hipStream_t st) {
   by_width(p.hdp, [&](auto ns) {
-    hipLaunchKernelGGL(k8_read<ns()>, dim3(nrows, p.n_kv), dim3(256), 0, st, p, rows, inl, k, v);
+    hipLaunchKernelGGL(k8_read<ns()>, dim3(nrows * p.n_kv), dim3(256), 0, st, p, rows, inl, k, v);
   });
   return hipGetLastError();
 }
