@@ -55,6 +55,37 @@ __device__ __forceinline__ float2 rotated(float x, float y, double c, double s) 
   return make_float2((float)(a * c - b * s), (float)(a * s + b * c));
 }
 
+// Whether this workgroup is the last of `n` to have written its part: the others' are then in
+// memory. Every thread calls it; `last` is a word of LDS. The last one sets the counter back for
+// the next call on the cache. Parts are written and read by accesses of device scope, which
+// go past the XCDs' own caches, so that all that is waited for is the workgroup's own stores (a fence of
+// that scope writes a whole cache back for every wave: 8 sequences at 65000 in 1630 us).
+__device__ __forceinline__ bool last_part(uint32_t* done, uint32_t n, uint32_t* last) {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    *last = atomicAdd(done, 1u) == n - 1 ? 1u : 0u;
+    if (*last) *done = 0;
+  }
+  __syncthreads();
+  return *last != 0;
+}
+__device__ __forceinline__ void store_shared2(float* p, float2 v) {
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), __builtin_bit_cast(uint64_t, v), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared2(const float* p) {
+  return __builtin_bit_cast(float2, __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+__device__ __forceinline__ void store_shared4(float* p, float4 v) {
+  store_shared2(p, make_float2(v.x, v.y));
+  store_shared2(p + 2, make_float2(v.z, v.w));
+}
+__device__ __forceinline__ float4 load_shared4(const float* p) {
+  const float2 a = load_shared2(p), b = load_shared2(p + 2);
+  return make_float4(a.x, a.y, b.x, b.y);
+}
+
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows of the caller's: any float's alignment
 __device__ __forceinline__ float4 load4(const float* p) {
   const f32x4u v = *reinterpret_cast<const f32x4u*>(p);
@@ -118,13 +149,16 @@ struct BlockRows {
       *reinterpret_cast<float4*>((value(i) ? vt : kt) + row(i) * hs + 4 * col(i)) = v[y];
     }
   }
-  // the first n rows to [2][n_kv][16][hd] at to (of kv head 0)
+  // the first n rows to [2][n_kv][16][hd] at to (of kv head 0); SHARED: for other workgroups of the launch
+  template <bool SHARED = false>
   __device__ __forceinline__ void put_global(const Kv8Pool& p, float* to, uint32_t h, uint32_t n) const {
 #pragma unroll
     for (uint32_t y = 0; y < NS; y++) {
       const uint32_t i = threadIdx.x + 256 * y, r = row(i), c = col(i);
-      if (r < n && 4 * c < p.hd)
-        *reinterpret_cast<float4*>(to + (((size_t)value(i) * p.n_kv + h) * kKv8Block + r) * p.hd + 4 * c) = v[y];
+      if (r >= n || 4 * c >= p.hd) continue;
+      float* d = to + (((size_t)value(i) * p.n_kv + h) * kKv8Block + r) * p.hd + 4 * c;
+      if (SHARED) store_shared4(d, v[y]);
+      else *reinterpret_cast<float4*>(d) = v[y];
     }
   }
   // the largest magnitudes of keys and values, as bits: a NaN's above infinity's above every
@@ -284,9 +318,9 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
 //     of block l / 16: a block's scale is a lane's scalar;
 //   O^T = V^T P^T: those 16 weights are the lane's own B operand as they stand, and the
 //     values' 16 bytes a dim are its A operand.
-// Codes go from memory to registers as the MFMAs want them, no LDS on the way. The parts' sums
-// are joined in a fixed order (k8_join), so a row's bits depend neither on the batch nor on
-// how many parts the call has.
+// Codes go from memory to registers as the MFMAs want them, no LDS on the way. The last
+// workgroup of a group to finish joins its parts, in their order, so a row's bits depend neither
+// on the batch nor on how the workgroups were scheduled.
 // ---------------------------------------------------------------------------------
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -355,7 +389,7 @@ constexpr uint32_t kBadRow = 0x7fc00000u;  // a part's maximum: a NaN or +inf sc
 
 // A row's mean over its span, column d: uniform weights (rare). vo: its own block's values.
 __device__ float uniform_mean(const Kv8Pool& p, uint32_t table, uint32_t h, uint32_t start, uint32_t pos, uint32_t d,
-                              const float* vo, uint32_t vstride) {
+                              const float* vo, uint32_t vstride, bool shared = false) {
   const uint32_t own = pos / kKv8Block * kKv8Block;
   double sum = 0.0;
   for (uint32_t b = start / kKv8Block; b * kKv8Block < own; b++) {
@@ -365,7 +399,7 @@ __device__ float uniform_mean(const Kv8Pool& p, uint32_t table, uint32_t h, uint
     for (uint32_t r = 0; r < kKv8Block; r++) n += b * kKv8Block + r >= start ? (int)c[r] - 128 : 0;
     sum += (double)n * (double)p.scales[2 * u + 1];
   }
-  for (uint32_t r = start > own ? start - own : 0; r <= pos - own; r++) sum += (double)vo[r * vstride + d];
+  for (uint32_t r = start > own ? start - own : 0; r <= pos - own; r++) sum += (double)(shared ? __hip_atomic_load(vo + r * vstride + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : vo[r * vstride + d]);
   return (float)(sum / (double)(pos + 1 - start));
 }
 
@@ -382,9 +416,67 @@ struct Kv8Part {
 __device__ __forceinline__ Kv8Part parts_of(const Kv8Args& a, float* o, uint32_t nparts, uint32_t nx, uint32_t R) {
   return {o, reinterpret_cast<float2*>(o + (size_t)nparts * nx * a.p.n_kv * R * a.p.hd), nx, a.p.n_kv, R};
 }
+// First position that a token attends to.
+__device__ __forceinline__ uint32_t kv8_start(const Kv8Args& a, uint32_t pos) {
+  return a.window && pos + 1 > a.window ? pos + 1 - a.window : 0;
+}
 __device__ __forceinline__ Kv8Part rows_parts(const Kv8Args& a, bool step) {
   const uint32_t G = a.n_heads / a.p.n_kv;
   return parts_of(a, a.part, a.nparts, step ? a.n : a.nrun, step ? G : kv8_group_tokens(G) * G);
+}
+
+// Sums of one row's four columns over parts: o and l in units of 2^m. A part's sums come times the
+// power that takes its maximum to the largest, rounded, then added; ok turns false at a maximum that
+// is a NaN.
+struct Joined {
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  float m = -INFINITY, l = 0.0f;
+  bool ok = true;
+  __device__ __forceinline__ void raise(float to) {
+    if (!(to > m)) return;
+    const float f = __builtin_amdgcn_exp2f(m - to);
+    l *= f;
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    m = to;
+  }
+  __device__ __forceinline__ void add(float pm, float pl, const float4& p) {  // pm at most m
+    if (!(pm > -INFINITY)) return;  // a part without a score: its sums may be unwritten
+    const float f = __builtin_amdgcn_exp2f(pm - m);
+    l += pl * f;
+    o = make_float4(o.x + p.x * f, o.y + p.y * f, o.z + p.z * f, o.w + p.w * f);
+  }
+  // parts s0 .. s1 - 1 in order, N of them loaded at a time. SHARED: from workgroups of this launch.
+  template <bool SHARED, uint32_t N>
+  __device__ __forceinline__ void parts(const Kv8Part& part, uint32_t s0, uint32_t s1, size_t row, uint32_t hd, uint32_t c) {
+    const size_t step = part.row(1, 0, 0, 0);
+    for (; s0 < s1; s0 += N) {
+      float2 v[N];
+      float4 w[N];
+      float mb = m;
+#pragma unroll
+      for (uint32_t k = 0; k < N; k++) {
+        v[k] = make_float2(-INFINITY, 0.0f);
+        if (s0 + k < s1) {
+          const float2* ml = part.ml + (s0 + k) * step + row;
+          const float* po = part.o + ((s0 + k) * step + row) * hd + 4 * c;
+          v[k] = SHARED ? load_shared2(reinterpret_cast<const float*>(ml)) : *ml;
+          w[k] = SHARED ? load_shared4(po) : *reinterpret_cast<const float4*>(po);
+        }
+        ok &= v[k].x == v[k].x;
+        mb = fmaxf(mb, v[k].x);
+      }
+      raise(mb);
+#pragma unroll
+      for (uint32_t k = 0; k < N; k++) add(v[k].x, v[k].y, w[k]);
+    }
+  }
+  __device__ __forceinline__ bool mean(float4& to) const {
+    to = make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
+    return ok && m > -INFINITY;
+  }
+};
+__device__ __forceinline__ void put_ctx(float* d, float4 v) {  // the caller's rows: any float's alignment
+  *reinterpret_cast<f32x4u*>(d) = f32x4u{v.x, v.y, v.z, v.w};
 }
 
 // LDS of k8_rows: queries, the own block's keys and values, its weights and sums, the waves' sums.
@@ -430,6 +522,67 @@ __device__ __forceinline__ bool step_part(const Kv8Args& a, const Kv8Inline& inl
   return false;
 }
 
+__device__ __forceinline__ float* ctx_row(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r) {
+  const uint32_t G = a.n_heads / a.p.n_kv;
+  return a.ctx + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * a.p.hd;
+}
+// Column c of a row whose weights are uniform (four columns; rare).
+template <bool STEP, bool SHARED>
+__device__ __forceinline__ float4 uniform_row(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r, uint32_t c) {
+  const Kv8Pool& p = a.p;
+  const uint32_t hd = p.hd, pos = run.pos0 + r / (a.n_heads / p.n_kv);
+  const float* vo = STEP ? kv8_open(p, run.table, h) + (size_t)p.n_kv * kKv8Block * hd
+                         : a.own + (((size_t)run.job * 2 + 1) * p.n_kv + h) * kKv8Block * hd;
+  float u[4];
+  for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, kv8_start(a, pos), pos, 4 * c + k, vo, hd, STEP && SHARED);
+  return make_float4(u[0], u[1], u[2], u[3]);
+}
+
+// grid (groups * n_kv * R), 256 threads: the context of one row of a group, joined from its
+// parts. kKv8Join parts at a time, in order, then what these give: in a call without this launch
+// (kv8_fused) there are no more than those.
+template <bool STEP>
+__global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
+  __shared__ float4 go[256];
+  __shared__ float gm[256], gl[256];
+  __shared__ uint32_t bad;
+  const Kv8Pool& p = a.p;
+  const Kv8Part part = rows_parts(a, STEP);
+  const uint32_t r = blockIdx.x % part.R, h = blockIdx.x / part.R % p.n_kv, x = blockIdx.x / part.R / p.n_kv;
+  Kv8Run run;
+  if (STEP) {
+    const AttnEntry e = a.ent ? a.ent[x] : inl.e[x];
+    run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
+  } else {
+    run = a.run[x];
+  }
+  const uint32_t t = threadIdx.x, hd = p.hd, q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
+  const uint32_t n = kv8_parts_of(run.pos0, kv8_start(a, run.pos0));
+  if (r >= run.n * (a.n_heads / p.n_kv)) return;
+  if (t == 0) bad = 0;
+  __syncthreads();
+  Joined all;
+  for (uint32_t s0 = 0; s0 < n; s0 += ng * kKv8Join) {
+    Joined j;
+    if (g < ng) j.parts<false, 8>(part, s0 + g * kKv8Join, min(n, s0 + (g + 1) * kKv8Join), part.row(0, x, h, r), hd, c);
+    if (!j.ok) bad = 1;
+    go[t] = j.o;
+    gm[t] = j.m;
+    gl[t] = j.l;
+    __syncthreads();
+    if (t < q4)
+      for (uint32_t k = 0; k < ng; k++) {
+        all.raise(gm[k * q4 + t]);
+        all.add(gm[k * q4 + t], gl[k * q4 + t], go[k * q4 + t]);
+      }
+    __syncthreads();
+  }
+  if (t >= q4) return;
+  float4 o;
+  if (!all.mean(o) || bad) o = uniform_row<STEP, false>(a, run, h, r, c);
+  put_ctx(ctx_row(a, run, h, r) + 4 * c, o);
+}
+
 // STEP: groups are entries, and the token is appended here. ONE: one workgroup takes both
 // the own block and what is before it (at most kKv8Split positions), and writes the context.
 // grid: (groups * n_kv, 1, parts), in a step without ONE (parts of all entries * n_kv). The kv
@@ -463,17 +616,35 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   float* ps = vt + kKv8Block * hs;               // [16][16]
   float* oo = ps + 16 * 16;                      // [rows][hs]
   float* wo = oo + rows * hs;                    // [4][rows][QS]
-  auto start_of = [&](uint32_t pos) { return a.window && pos + 1 > a.window ? pos + 1 - a.window : 0; };
+  auto start_of = [&](uint32_t pos) { return kv8_start(a, pos); };
   const uint32_t own = run.pos0 / kKv8Block * kKv8Block, last = run.pos0 + run.n - 1;
   const uint32_t base = start_of(run.pos0) / kKv8Block * kKv8Block;
   const uint32_t lo = base + (ONE || z == 0 ? 0 : z - 1) * kKv8Split, hi = min(own, lo + kKv8Split);
   const Kv8Part part = rows_parts(a, STEP);
   auto prow = [&](uint32_t r) { return part.row(z, x, h, r); };
-  if (!ONE && z && lo >= hi) {  // a call's group without that part
-    if (t < rows) part.ml[prow(t)] = make_float2(-INFINITY, 0.0f);
-    return;
-  }
+  if (!ONE && z && lo >= hi) return;  // a call's group without that part
   const bool mine = ONE || z == 0;
+  auto done = [&] {  // the last of the group's workgroups joins its parts; otherwise k8_join does
+    if (!a.fused) return;
+    if (last_part(a.done + (size_t)x * p.n_kv + h, kv8_parts_of(run.pos0, start_of(run.pos0)), &red[0]))
+      for (uint32_t i = t; i < rows * Q4; i += 256) {
+        const uint32_t r = i / Q4, c = i % Q4;
+        if (4 * c >= hd) continue;
+        Joined j;
+        j.parts<true, 8>(part, 0, kv8_parts_of(run.pos0, start_of(run.pos0)), part.row(0, x, h, r), hd, c);
+        float4 o;
+        if (!j.mean(o)) o = uniform_row<STEP, true>(a, run, h, r, c);
+        put_ctx(ctx_row(a, run, h, r) + 4 * c, o);
+      }
+  };
+  auto put4 = [&](float* d, float4 v) {
+    if (a.fused) store_shared4(d, v);
+    else *reinterpret_cast<float4*>(d) = v;
+  };
+  auto put2 = [&](float2* d, float2 v) {
+    if (a.fused) store_shared2(reinterpret_cast<float*>(d), v);
+    else *d = v;
+  };
   // the first tile's codes on their way before the queries are turned
   const uint8_t *ka = nullptr, *va = nullptr;
   float sk = 0.0f, sv = 0.0f;
@@ -556,7 +727,7 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
   if (mine) {
     if (STEP) {
       ob.turn_keys(p, block, r0, 1);
-      ob.put_global(p, p.open + (size_t)run.table * 2 * p.n_kv * kKv8Block * hd, h, r0 + 1);
+      ob.template put_global<!ONE>(p, p.open + (size_t)run.table * 2 * p.n_kv * kKv8Block * hd, h, r0 + 1);
     }
     ob.put(kt, vt, hs);
     if (STEP && r0 == kKv8Block - 1) {
@@ -599,15 +770,21 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
       }
     }
     __syncthreads();
-    for (uint32_t y = t; y < rows * hd; y += 256) {
-      const uint32_t r = y / hd, d = y % hd, pr = run.pos0 + r / G, st = start_of(pr);
-      float o = 0.0f;
-      for (uint32_t j = st > own ? st - own : 0; j <= pr - own; j++) o = fmaf(ps[r * 16 + j], vt[j * hs + d], o);
-      if (ONE) oo[r * hs + d] = o;
-      else part.o[prow(r) * hd + d] = o;
+    for (uint32_t y = t; y < rows * Q4; y += 256) {
+      const uint32_t r = y / Q4, d = 4 * (y % Q4), pr = run.pos0 + r / G, st = start_of(pr);
+      if (d >= hd) continue;
+      float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      for (uint32_t j = st > own ? st - own : 0; j <= pr - own; j++) {
+        const float w = ps[r * 16 + j];
+        const float4 v = *reinterpret_cast<const float4*>(vt + j * hs + d);
+        o = make_float4(fmaf(w, v.x, o.x), fmaf(w, v.y, o.y), fmaf(w, v.z, o.z), fmaf(w, v.w, o.w));
+      }
+      if (ONE) *reinterpret_cast<float4*>(oo + r * hs + d) = o;
+      else put4(part.o + prow(r) * hd + d, o);
     }
     if (!ONE) {
-      if (t < rows) part.ml[prow(t)] = make_float2(own_m[t], own_l[t]);
+      if (t < rows) put2(part.ml + prow(t), make_float2(own_m[t], own_l[t]));
+      done();
       return;
     }
   }
@@ -770,9 +947,14 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
           make_float4(o[d][0] * fo, o[d][1] * fo, o[d][2] * fo, o[d][3] * fo);
   }
   __syncthreads();
-  for (uint32_t y = t; y < rows * hd; y += 256) {
-    const uint32_t r = y / hd, d = y % hd;
-    float m = -INFINITY, l = 0.0f, v = 0.0f;
+  for (uint32_t y = t; y < rows * Q4; y += 256) {
+    const uint32_t r = y / Q4, d = 4 * (y % Q4);
+    if (d >= hd) continue;
+    float m = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [&](float4& to, const float4& w, float f) {
+      to = make_float4(to.x + w.x * f, to.y + w.y * f, to.z + w.z * f, to.w + w.w * f);
+    };
     bool bd = false;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
@@ -785,120 +967,129 @@ __global__ void __launch_bounds__(256, NS <= 6 ? 2 : 1) k8_rows(Kv8Args a, Kv8In
         if (!(wm[w][r] > -INFINITY)) continue;
         const float f = __builtin_amdgcn_exp2f(wm[w][r] - m);
         l += wl[w][r] * f;
-        v += wo[(w * rows + r) * QS + d] * f;
+        add(v, *reinterpret_cast<const float4*>(wo + (w * rows + r) * QS + d), f);
       }
     if (bd) m = __uint_as_float(kBadRow);
     if (!ONE) {
-      part.o[prow(r) * hd + d] = v;
-      if (d == 0) part.ml[prow(r)] = make_float2(m, l);
+      put4(part.o + prow(r) * hd + d, v);
+      if (d == 0) put2(part.ml + prow(r), make_float2(m, l));
       continue;
     }
-    // the own block's part and this one, as k8_join joins parts
+    // the own block's part and this one, as Joined adds them
     const float m0 = own_m[r], mm = fmaxf(m0, m);
     const uint32_t pr = run.pos0 + r / G;
-    float c;
+    float4 c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (bd || m0 != m0 || mm == -INFINITY) {
-      c = uniform_mean(p, run.table, h, start_of(pr), pr, d, vt, hs);
+      float u[4];
+      for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, start_of(pr), pr, d + k, vt, hs);
+      c = make_float4(u[0], u[1], u[2], u[3]);
     } else {
-      float la = 0.0f, oa = 0.0f, lb = 0.0f, ob = 0.0f;
+      float ls = 0.0f;
       if (m0 > -INFINITY) {
         const float f = __builtin_amdgcn_exp2f(m0 - mm);
-        la += own_l[r] * f;
-        oa += oo[r * hs + d] * f;
+        ls += own_l[r] * f;
+        add(c, *reinterpret_cast<const float4*>(oo + r * hs + d), f);
       }
       if (m > -INFINITY) {
         const float f = __builtin_amdgcn_exp2f(m - mm);
-        lb += l * f;
-        ob += v * f;
+        ls += l * f;
+        add(c, v, f);
       }
-      c = (oa + ob) / (la + lb);
+      c = make_float4(c.x / ls, c.y / ls, c.z / ls, c.w / ls);
     }
-    a.ctx[((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd + d] = c;
+    put_ctx(ctx_row(a, run, h, r) + d, c);
   }
+  if (!ONE) done();
 }
 
-// grid (groups, n_kv R), 256 threads: a row's parts joined, threads of several groups taking
-// every ng-th part for four columns each, the groups then added in order.
-template <bool STEP>
-__global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
-  __shared__ float4 go[256];
-  __shared__ float gl[256], gm[4];
+// One row again, by the first 256 threads of the workgroup (all of which call it), in f32: 64
+// positions at a time, four threads a score. ls: 64 floats, po: 256 float4 of LDS. Threads
+// t < hd / 4 return the row's columns 4 t .. 4 t + 3.
+__device__ __forceinline__ float4 row_again(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r, float* ls, float4* po) {
   const Kv8Pool& p = a.p;
-  const uint32_t x = blockIdx.x, t = threadIdx.x, hd = p.hd, q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
-  const uint32_t G = a.n_heads / p.n_kv;
-  const Kv8Part part = rows_parts(a, STEP);
-  const uint32_t h = blockIdx.y / part.R, r = blockIdx.y % part.R;
-  Kv8Run run;
-  if (STEP) {
-    const AttnEntry e = a.ent ? a.ent[x] : inl.e[x];
-    run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
-  } else {
-    run = a.run[x];
-  }
-  if (r >= run.n * G) return;
-  const size_t rows = (size_t)part.nx * part.n_kv * part.R, row = part.row(0, x, h, r);
-  const uint32_t nparts = STEP ? kv8_parts_of(run.pos0, a.window && run.pos0 + 1 > a.window ? run.pos0 + 1 - a.window : 0) : a.nparts;
-  float m = -INFINITY;
-  bool bad = false;
-  for (uint32_t s = t; s < nparts; s += 256) {
-    const float v = part.ml[s * rows + row].x;
-    bad |= v != v;
-    m = fmaxf(m, v);
-  }
-  m = wave64_max(m);
-  if (__ballot(bad)) m = INFINITY;  // no part's maximum is: the mark
-  if ((t & 63) == 0) gm[t >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(gm[0], gm[1]), fmaxf(gm[2], gm[3]));
-  const bool uniform = m == INFINITY || m == -INFINITY;
-  float l = 0.0f;
+  const uint32_t t = threadIdx.x, lane = t & 63, hd = p.hd, G = a.n_heads / p.n_kv, pos = run.pos0 + r / G;
+  const uint32_t start = kv8_start(a, pos), own = pos / kKv8Block * kKv8Block;
+  const float* q = a.qr + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd;
+  const uint32_t job = run.job + pos / kKv8Block - run.pos0 / kKv8Block;
+  const float* ko = a.own + ((size_t)job * 2 * p.n_kv + h) * kKv8Block * hd;
+  const float* vo = ko + (size_t)p.n_kv * kKv8Block * hd;
+  const uint32_t q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
+  float M = -INFINITY, L = 0.0f;
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (g < ng && !uniform)
-    for (uint32_t s0 = g; s0 < nparts; s0 += 4 * ng) {
-      float2 v[4];
-      float4 w[4];
-#pragma unroll
-      for (uint32_t k = 0; k < 4; k++) {
-        const uint32_t s = s0 + k * ng;
-        v[k] = make_float2(-INFINITY, 0.0f);
-        if (s < nparts) {
-          v[k] = part.ml[s * rows + row];
-          w[k] = reinterpret_cast<const float4*>(part.o + (s * rows + row) * hd)[c];
+  bool uniform = false;
+  for (uint32_t c0 = start / kKv8Block * kKv8Block; c0 <= pos && !uniform; c0 += 64) {
+    const uint32_t pk = c0 + t / 4;
+    float s = 0.0f;
+    const bool in = pk >= start && pk <= pos;
+    if (in && t < 256) {
+      const size_t u = pk < own ? kv8_block(p, kv8_page(p, run.table, pk / kKv8Block), pk / kKv8Block, h) : 0;
+      for (uint32_t d = t % 4; d < hd; d += 4)
+        s = fmaf(q[d], pk < own ? (float)((int)kv8_codes(p, u)[kv8_key(p.hdp, pk % kKv8Block, d)] - 128) : ko[(pk - own) * hd + d], s);
+      if (pk < own) s *= p.scales[2 * u];
+    }
+    s += __shfl_xor(s, 1, 64);
+    s += __shfl_xor(s, 2, 64);
+    __syncthreads();
+    if (t < 256 && t % 4 == 0) ls[t / 4] = in ? s * (a.scale * kLog2e) : -INFINITY;
+    __syncthreads();
+    const float v = ls[lane];
+    if (__ballot(v != v || v == INFINITY)) uniform = true;  // every wave sees the same scores
+    const float mc = wave64_max(v);
+    if (uniform || mc == -INFINITY) continue;
+    const float mn = fmaxf(M, mc), f = __builtin_amdgcn_exp2f(M - mn), pv = __builtin_amdgcn_exp2f(v - mn);
+    M = mn;
+    L = L * f + wave64_sum(pv);
+    __syncthreads();
+    if (t < 64) ls[t] = pv;
+    __syncthreads();
+    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+    if (g < ng)
+      for (uint32_t j = g; j < 64; j += ng) {
+        const uint32_t pj = c0 + j;
+        if (pj < start || pj > pos) continue;
+        const float w = ls[j];
+        float4 b;
+        if (pj < own) {
+          const size_t u = kv8_block(p, kv8_page(p, run.table, pj / kKv8Block), pj / kKv8Block, h);
+          const uint8_t* cv = kv8_codes(p, u) + kKv8Block * p.hdp + pj % kKv8Block;
+          const float sv = p.scales[2 * u + 1];
+          auto at = [&](uint32_t d) { return (float)((int)cv[d * kKv8Block] - 128) * sv; };
+          b = make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
+        } else {
+          b = *reinterpret_cast<const float4*>(vo + (pj - own) * hd + 4 * c);
         }
+        o = make_float4(fmaf(w, b.x, o.x), fmaf(w, b.y, o.y), fmaf(w, b.z, o.z), fmaf(w, b.w, o.w));
       }
-#pragma unroll
-      for (uint32_t k = 0; k < 4; k++) {
-        if (!(v[k].x > -INFINITY)) continue;
-        const float f = __builtin_amdgcn_exp2f(v[k].x - m);
-        l += v[k].y * f;
-        o = make_float4(o.x + w[k].x * f, o.y + w[k].y * f, o.z + w[k].z * f, o.w + w[k].w * f);
-      }
-    }
-  go[t] = o;
-  gl[t] = l;
-  __syncthreads();
-  if (t >= q4) return;
-  if (!uniform) {
-    for (uint32_t k = 1; k < ng; k++) {
-      const float4 b = go[k * q4 + t];
-      l += gl[k * q4 + t];
-      o = make_float4(o.x + b.x, o.y + b.y, o.z + b.z, o.w + b.w);
-    }
-    o = make_float4(o.x / l, o.y / l, o.z / l, o.w / l);
-  } else {
-    const uint32_t pos = run.pos0 + r / G;
-    const float* vo = STEP ? kv8_open(p, run.table, h) + (size_t)p.n_kv * kKv8Block * hd
-                           : a.own + (((size_t)run.job * 2 + 1) * p.n_kv + h) * kKv8Block * hd;
-    const uint32_t start = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0;
+  }
+  if (uniform || M == -INFINITY) {
+    if (t >= q4) return o;
     float u[4];
     for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, start, pos, 4 * t + k, vo, hd);
-    o = make_float4(u[0], u[1], u[2], u[3]);
+    return make_float4(u[0], u[1], u[2], u[3]);
   }
-  float* dst = a.ctx + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd + 4 * t;
-  dst[0] = o.x;
-  dst[1] = o.y;
-  dst[2] = o.z;
-  dst[3] = o.w;
+  __syncthreads();
+  if (t < 256) po[t] = o;
+  __syncthreads();
+  if (t < q4) {
+    for (uint32_t k = 1; k < ng; k++) {
+      const float4 b = po[k * q4 + t];
+      o = make_float4(o.x + b.x, o.y + b.y, o.z + b.z, o.w + b.w);
+    }
+    o = make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
+  }
+  return o;
+}
+
+// The rows r0 + i of the bits i that are set in marks [8].
+__device__ __forceinline__ void rows_again(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r0, const uint32_t* marks, float* ls,
+                           float4* po) {
+  for (uint32_t k = 0; k < 8; k++)
+    for (uint32_t left = marks[k]; left; left &= left - 1) {
+      const uint32_t r = r0 + 32 * k + __builtin_ctz(left), t = threadIdx.x;
+      const float4 v = row_again(a, run, h, r, ls, po);
+      if (t < a.p.hd / 4) put_ctx(ctx_row(a, run, h, r) + 4 * t, v);
+      __syncthreads();
+    }
 }
 
 // ---------------------------------------------------------------------------------
@@ -942,6 +1133,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
   __shared__ u32x4 qlo[8 * KS * 64];  // the queries' second halves: in registers they would spill
   __shared__ float2 sc[2][4];
+  __shared__ uint32_t marks[8];  // rows to be summed again, a bit each
   const Kv8Pool& p = a.p;
   const uint32_t h = blockIdx.x, x = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
   const uint32_t lane = t & 63, l32 = lane & 31, hf = lane >> 5;
@@ -950,7 +1142,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   const Kv8Run* T = a.run + a.nrun + x;
   const uint32_t i0 = uni(T->i0), ntok = uni(T->n), pos0 = uni(T->pos0), table = uni(T->table), job0 = uni(T->job);
   const uint32_t rows = ntok * G, last = pos0 + ntok - 1;
-  auto start_of = [&](uint32_t pos) { return a.window && pos + 1 > a.window ? pos + 1 - a.window : 0; };
+  auto start_of = [&](uint32_t pos) { return kv8_start(a, pos); };
   auto own_of = [](uint32_t pos) { return pos / kKv8Block * kKv8Block; };
   const uint32_t base = own_of(start_of(pos0)), lo = base + z * a.tkeys, hi = min(own_of(last), lo + a.tkeys);
   const uint32_t row = 32 * wave + l32, rr = min(row, rows - 1), pos = pos0 + rr / G;
@@ -958,10 +1150,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   const Kv8Part part = tile_parts(a);
   const size_t prow = part.row(z, x, h, row);  // 256 rows a kv head
   const bool mine = row < rows, busy = 32 * wave < rows;
-  if (z && lo >= hi) {
-    if (mine && hf == 0) part.ml[prow] = make_float2(-INFINITY, 0.0f);
-    return;
-  }
+  if (z && lo >= hi) return;
   // what the wave's rows attend to of the held blocks: from its first row's start to its last row's own block
   const uint32_t pw0 = pos0 + min(32 * wave, rows - 1) / G, pw1 = pos0 + min(32 * wave + 31, rows - 1) / G;
   const uint32_t w_lo = start_of(pw0), w_hi = min(own_of(pw1), hi), w_in0 = start_of(pw1), w_in1 = min(own_of(pw0), hi);
@@ -1281,152 +1470,67 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   }
   odd = max32(odd ? 1.0f : 0.0f) != 0.0f || L != L || M == INFINITY;
   const float fo = pow2(ev);
-  if (mine) {
+  auto four = [&](uint32_t d, uint32_t j, float f) {  // columns 32 d + 8 j + 4 hf on
+    return make_float4(o[d][4 * j] * f, o[d][4 * j + 1] * f, o[d][4 * j + 2] * f, o[d][4 * j + 3] * f);
+  };
+  if (a.tsplits > 1) {
+    if (!mine) return;
     if (hf == 0) part.ml[prow] = make_float2(odd ? __uint_as_float(kBadRow) : M, L);
 #pragma unroll
     for (uint32_t d = 0; d < NS; d++)
 #pragma unroll
       for (uint32_t j = 0; j < 4; j++) {
         const uint32_t c = 32 * d + 8 * j + 4 * hf;
-        if (c < hd)
-          *reinterpret_cast<float4*>(part.o + prow * hd + c) =
-              make_float4(o[d][4 * j] * fo, o[d][4 * j + 1] * fo, o[d][4 * j + 2] * fo, o[d][4 * j + 3] * fo);
+        if (c < hd) *reinterpret_cast<float4*>(part.o + prow * hd + c) = four(d, j, fo);
+      }
+    return;
+  }
+  // the only split: the context itself
+  if (t < 8) marks[t] = 0;
+  __syncthreads();
+  const Kv8Run run{i0, ntok, pos0, job0, table};
+  if (mine) {
+    const bool again = odd || M == -INFINITY;
+    if (again && hf == 0) atomicOr(&marks[row / 32], 1u << (row % 32));
+#pragma unroll
+    for (uint32_t d = 0; d < NS; d++)
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t c = 32 * d + 8 * j + 4 * hf;
+        const float4 v = four(d, j, fo);
+        if (c < hd && !again) put_ctx(ctx_row(a, run, h, row) + c, make_float4(v.x / L, v.y / L, v.z / L, v.w / L));
       }
   }
+  __syncthreads();
+  rows_again(a, run, h, 0, marks, reinterpret_cast<float*>(lds + 4096), reinterpret_cast<float4*>(lds));
 }
 
-// One row again, by the workgroup, in f32: 64 positions at a time, four threads a score. ls: 64
-// floats, po: 256 float4 of LDS. Threads t < hd / 4 return the row's columns 4 t .. 4 t + 3.
-__device__ float4 row_again(const Kv8Args& a, const Kv8Run& run, uint32_t h, uint32_t r, float* ls, float4* po) {
-  const Kv8Pool& p = a.p;
-  const uint32_t t = threadIdx.x, lane = t & 63, hd = p.hd, G = a.n_heads / p.n_kv, pos = run.pos0 + r / G;
-  const uint32_t start = a.window && pos + 1 > a.window ? pos + 1 - a.window : 0, own = pos / kKv8Block * kKv8Block;
-  const float* q = a.qr + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd;
-  const uint32_t job = run.job + pos / kKv8Block - run.pos0 / kKv8Block;
-  const float* ko = a.own + ((size_t)job * 2 * p.n_kv + h) * kKv8Block * hd;
-  const float* vo = ko + (size_t)p.n_kv * kKv8Block * hd;
-  const uint32_t q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
-  float M = -INFINITY, L = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  bool uniform = false;
-  for (uint32_t c0 = start / kKv8Block * kKv8Block; c0 <= pos && !uniform; c0 += 64) {
-    const uint32_t pk = c0 + t / 4;
-    float s = 0.0f;
-    const bool in = pk >= start && pk <= pos;
-    if (in) {
-      const size_t u = pk < own ? kv8_block(p, kv8_page(p, run.table, pk / kKv8Block), pk / kKv8Block, h) : 0;
-      for (uint32_t d = t % 4; d < hd; d += 4)
-        s = fmaf(q[d], pk < own ? (float)((int)kv8_codes(p, u)[kv8_key(p.hdp, pk % kKv8Block, d)] - 128) : ko[(pk - own) * hd + d], s);
-      if (pk < own) s *= p.scales[2 * u];
-    }
-    s += __shfl_xor(s, 1, 64);
-    s += __shfl_xor(s, 2, 64);
-    __syncthreads();
-    if (t % 4 == 0) ls[t / 4] = in ? s * (a.scale * kLog2e) : -INFINITY;
-    __syncthreads();
-    const float v = ls[lane];
-    if (__ballot(v != v || v == INFINITY)) uniform = true;  // every wave sees the same scores
-    const float mc = wave64_max(v);
-    if (uniform || mc == -INFINITY) continue;
-    const float mn = fmaxf(M, mc), f = __builtin_amdgcn_exp2f(M - mn), pv = __builtin_amdgcn_exp2f(v - mn);
-    M = mn;
-    L = L * f + wave64_sum(pv);
-    __syncthreads();
-    if (t < 64) ls[t] = pv;
-    __syncthreads();
-    o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
-    if (g < ng)
-      for (uint32_t j = g; j < 64; j += ng) {
-        const uint32_t pj = c0 + j;
-        if (pj < start || pj > pos) continue;
-        const float w = ls[j];
-        float4 b;
-        if (pj < own) {
-          const size_t u = kv8_block(p, kv8_page(p, run.table, pj / kKv8Block), pj / kKv8Block, h);
-          const uint8_t* cv = kv8_codes(p, u) + kKv8Block * p.hdp + pj % kKv8Block;
-          const float sv = p.scales[2 * u + 1];
-          auto at = [&](uint32_t d) { return (float)((int)cv[d * kKv8Block] - 128) * sv; };
-          b = make_float4(at(4 * c), at(4 * c + 1), at(4 * c + 2), at(4 * c + 3));
-        } else {
-          b = *reinterpret_cast<const float4*>(vo + (pj - own) * hd + 4 * c);
-        }
-        o = make_float4(fmaf(w, b.x, o.x), fmaf(w, b.y, o.y), fmaf(w, b.z, o.z), fmaf(w, b.w, o.w));
-      }
-  }
-  if (uniform || M == -INFINITY) {
-    if (t >= q4) return o;
-    float u[4];
-    for (uint32_t k = 0; k < 4; k++) u[k] = uniform_mean(p, run.table, h, start, pos, 4 * t + k, vo, hd);
-    return make_float4(u[0], u[1], u[2], u[3]);
-  }
-  __syncthreads();
-  po[t] = o;
-  __syncthreads();
-  if (t < q4) {
-    for (uint32_t k = 1; k < ng; k++) {
-      const float4 b = po[k * q4 + t];
-      o = make_float4(o.x + b.x, o.y + b.y, o.z + b.z, o.w + b.w);
-    }
-    o = make_float4(o.x / L, o.y / L, o.z / L, o.w / L);
-  }
-  return o;
-}
-
-// grid (tiles, n_kv, ceil(256 / rows a workgroup)), 256 threads: the splits of a tile's rows
-// joined, a thread per four columns of a row.
+// grid (tiles * n_kv, 256 / rows a workgroup), 256 threads: the splits of a tile's rows joined,
+// a thread per four columns of a row.
 __global__ void __launch_bounds__(256) k8_join_tile(Kv8Args a) {
   __shared__ float4 po[256];
   __shared__ float ls[64];
   __shared__ uint32_t marks[8];
   const Kv8Pool& p = a.p;
-  const uint32_t x = blockIdx.x, h = blockIdx.y, t = threadIdx.x, hd = p.hd, q4 = hd / 4, rpw = 256 / q4, G = a.n_heads / p.n_kv;
+  const uint32_t x = blockIdx.x / p.n_kv, h = blockIdx.x % p.n_kv, t = threadIdx.x, hd = p.hd, q4 = hd / 4, rpw = 256 / q4;
+  const uint32_t G = a.n_heads / p.n_kv;
   const Kv8Run run = a.run[a.nrun + x];
   const Kv8Part part = tile_parts(a);
-  const uint32_t r0 = blockIdx.z * rpw, r = r0 + t / q4, c = t % q4, rows = run.n * G;
+  const uint32_t r0 = blockIdx.y * rpw, r = r0 + t / q4, c = t % q4, rows = run.n * G;
   if (r0 >= rows) return;
-  const bool mine = t / q4 < rpw && r < rows;
-  auto dst = [&](uint32_t r) { return a.ctx + ((size_t)(run.i0 + r / G) * a.n_heads + h * G + r % G) * hd; };
-  auto put = [&](float* d, float4 v) {
-    d[0] = v.x;
-    d[1] = v.y;
-    d[2] = v.z;
-    d[3] = v.w;
-  };
   if (t < 8) marks[t] = 0;
   __syncthreads();
-  if (mine) {
-    const size_t step = (size_t)part.nx * part.n_kv * part.R, row = part.row(0, x, h, r);
-    float m = -INFINITY, l = 0.0f;
-    bool again = false;
-    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (uint32_t s = 0; s < a.tsplits; s++) {
-      const float v = part.ml[s * step + row].x;
-      again |= v != v;
-      m = fmaxf(m, v);
-    }
-    again |= m == -INFINITY;
-    if (!again) {
-      for (uint32_t s = 0; s < a.tsplits; s++) {
-        const float2 v = part.ml[s * step + row];
-        if (!(v.x > -INFINITY)) continue;
-        const float f = __builtin_amdgcn_exp2f(v.x - m);
-        const float4 w = reinterpret_cast<const float4*>(part.o + (s * step + row) * hd)[c];
-        l += v.y * f;
-        o = make_float4(o.x + w.x * f, o.y + w.y * f, o.z + w.z * f, o.w + w.w * f);
-      }
-      put(dst(r) + 4 * c, make_float4(o.x / l, o.y / l, o.z / l, o.w / l));
-    } else if (c == 0) {
-      atomicOr(&marks[t / q4 / 32], 1u << (t / q4 % 32));
-    }
+  if (t / q4 < rpw && r < rows) {
+    const uint32_t last = run.pos0 + run.n - 1, first = kv8_start(a, run.pos0);
+    const uint32_t n = max(1u, (last / kKv8Block * kKv8Block - first / kKv8Block * kKv8Block + a.tkeys - 1) / a.tkeys);
+    Joined j;
+    j.parts<false, 2>(part, 0, n, part.row(0, x, h, r), hd, c);
+    float4 v;
+    if (j.mean(v)) put_ctx(ctx_row(a, run, h, r) + 4 * c, v);
+    else if (c == 0) atomicOr(&marks[(r - r0) / 32], 1u << ((r - r0) % 32));
   }
   __syncthreads();
-  for (uint32_t k = 0; k < 8; k++)
-    for (uint32_t left = marks[k]; left; left &= left - 1) {
-      const uint32_t r1 = r0 + 32 * k + __builtin_ctz(left);
-      const float4 v = row_again(a, run, h, r1, ls, po);
-      if (t < q4) put(dst(r1) + 4 * t, v);
-      __syncthreads();
-    }
+  rows_again(a, run, h, r0, marks, ls, po);
 }
 
 // grid (chunks * n_kv), 256 threads: rows of one block, from its codes or from the open rows.
@@ -1495,20 +1599,6 @@ __global__ void __launch_bounds__(256) k8_reopen(Kv8Pool p, Kv8RowsInline inl) {
   }
 }
 
-bool overlaps(const float* a, size_t na, const float* b, size_t nb) { return a < b + nb && b < a + na; }
-
-// One workgroup a group and kv head: everything before the own block fits one part, and no
-// other workgroup's input lies under the context (a call reads its own in the launch before).
-bool one_part(const Kv8Args& a, bool step) {
-  const size_t n = a.n, qd = (size_t)a.n_heads * a.p.hd, kvd = (size_t)a.p.n_kv * a.p.hd;
-  const size_t more = a.nsl > 1 ? (a.nsl - 1) * a.sl_stride : 0;
-  auto over = [&](const float* p, size_t width, size_t stride) {
-    return overlaps(a.ctx, n * qd, p, (n - 1) * stride + width + more);
-  };
-  if (a.nparts != 2) return false;
-  return !step || (!over(a.q, qd, a.q_stride) && !over(a.k, kvd, a.kv_stride) && !over(a.v, kvd, a.kv_stride));
-}
-
 template <int NS, bool STEP>
 void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
   // what 16 rows of the widest heads of this build take, set once; a call asks for its own rows'
@@ -1518,13 +1608,13 @@ void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
            hipFuncSetAttribute((const void*)k8_rows<NS, STEP, false>, hipFuncAttributeMaxDynamicSharedMemorySize, most) == hipSuccess;
   }();
   (void)set;
-  const bool one = one_part(a, STEP);
+  const bool one = a.nparts == 2;  // one workgroup a group and kv head
   const uint32_t G = a.n_heads / a.p.n_kv, rows = STEP ? G : kv8_group_tokens(G) * G, nx = STEP ? a.n : a.nrun;
   const uint32_t lds = kv8_rows_lds(a.p.hdp, rows);
   const dim3 grid(a.p.n_kv * (STEP && !one ? a.items : nx), 1, STEP || one ? 1 : a.nparts);
   auto kernel = one ? k8_rows<NS, STEP, true> : k8_rows<NS, STEP, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, inl);
-  if (!one) hipLaunchKernelGGL(k8_join<STEP>, dim3(nx, a.p.n_kv * rows), dim3(256), 0, st, a, inl);
+  if (!one && !a.fused) hipLaunchKernelGGL(k8_join<STEP>, dim3(a.p.n_kv * nx * rows), dim3(256), 0, st, a, inl);
 }
 
 // f of the build for the heads' width
@@ -1556,14 +1646,15 @@ hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
   if (!a.ctx) return hipGetLastError();
   if (a.ntile) {
     const dim3 grid(a.p.n_kv, a.ntile, a.tsplits);
+    const uint32_t rpw = 256 / (a.p.hd / 4);
     switch (a.p.hdp / 32) {
       case 1: hipLaunchKernelGGL(k8_tile<1>, grid, dim3(512), 0, st, a); break;
       case 2: hipLaunchKernelGGL(k8_tile<2>, grid, dim3(512), 0, st, a); break;
       case 3: hipLaunchKernelGGL(k8_tile<3>, grid, dim3(512), 0, st, a); break;
       default: hipLaunchKernelGGL(k8_tile<4>, grid, dim3(512), 0, st, a); break;
     }
-    const uint32_t rpw = 256 / (a.p.hd / 4);
-    hipLaunchKernelGGL(k8_join_tile, dim3(a.ntile, a.p.n_kv, (kKv8TileRows + rpw - 1) / rpw), dim3(256), 0, st, a);
+    if (a.tsplits > 1)
+      hipLaunchKernelGGL(k8_join_tile, dim3(a.ntile * a.p.n_kv, (kKv8TileRows + rpw - 1) / rpw), dim3(256), 0, st, a);
   }
   return a.nrun ? launch_rows_of<false>(a, Kv8Inline{}, st) : hipGetLastError();
 }

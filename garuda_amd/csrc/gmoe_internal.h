@@ -512,6 +512,15 @@ struct Kv8Rows {
 // one is the row's own block; the others begin at a block's start).
 constexpr uint32_t kKv8Split = 512;
 constexpr uint32_t kv8_parts(uint32_t span) { return 1 + (span + kKv8Block - 1 + kKv8Split - 1) / kKv8Split; }
+// Whether the workgroup that finishes last joins a group's parts, or a launch of its own: while
+// a call's workgroups all run at once, and the join is one pass over a few parts, it costs less
+// than a launch (one sequence at 4000: 15.7 us, 18.1 with the launch; 8 at 2047 20.5 and 21.4);
+// beyond that, writing the parts past the caches and counting them costs every workgroup more
+// (8 sequences at 65000 248 us, 222 with the launch; 32 with 8 heads of 256 on one at 6000 29.7 and 27.9).
+constexpr uint32_t kKv8Join = 16, kKv8FusedWgs = 1024;
+constexpr uint32_t kv8_fused(uint32_t items, uint32_t n_kv, uint32_t nparts, uint32_t floats) {  // of a group's context
+  return nparts <= kKv8Join && floats <= 4 * 256 && (uint64_t)items * n_kv <= kKv8FusedWgs ? 1 : 0;
+}
 constexpr uint32_t kv8_parts_of(uint32_t pos, uint32_t start) {  // of an entry
   return 1 + (pos / kKv8Block * kKv8Block - start / kKv8Block * kKv8Block + kKv8Split - 1) / kKv8Split;
 }
@@ -538,7 +547,9 @@ struct Kv8Args {
   float2* own_max;     //   and [njob][n_kv] their largest magnitudes (keys, values)
   float* part;         // partial sums of the groups' rows (kv8_part_floats): the own block,
   uint32_t nparts;     //   then as many splits as the longest span has
-  uint32_t items;      // a step's parts, over all entries
+  uint32_t* done;      // [groups][n_kv] parts that are written; 0 between calls
+  uint32_t fused;      // 1: the last workgroup of a group joins its parts (kv8_fused)
+  uint32_t items;      // the groups' parts, over all entries
   float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions
   uint32_t tsplits, tkeys;
 };

@@ -88,6 +88,9 @@ struct gmoe_kv {
   std::vector<Seq> seqs;
   uint8_t* scratch = nullptr; // per call: entries, rotated q, chunk partials
   size_t scratch_bytes = 0;
+  uint32_t* done = nullptr;   // 8 bits: counters of written parts (Kv8Args), 0 between calls
+  size_t n_done = 0;
+  uintptr_t scratch_id = 0;   // another one whenever scratch or done moves
   // pinned staging of the entries and tiles of calls above kAttnInline tokens: two halves,
   // each taken from its start to its end; a half's event says its calls have read it
   uint8_t* pin = nullptr;
@@ -106,6 +109,7 @@ struct gmoe_kv {
     if (p8.open) hipFree(p8.open);
     if (p8.turns) hipFree(const_cast<double*>(p8.turns));
     if (saved) hipFree(saved);
+    if (done) hipFree(done);
     if (scratch) hipFree(scratch);
     if (pin) hipHostFree(pin);
     for (auto& e : pin_ev)
@@ -122,8 +126,26 @@ gmoe_status grow_scratch(gmoe_kv* kv, size_t bytes) {
   kv->scratch = nullptr;
   kv->scratch_bytes = 0;
   const size_t want = std::max(bytes, (size_t)8 << 20);
+  kv->scratch_id++;
   KV_TRY(hipMalloc(&kv->scratch, want));
   kv->scratch_bytes = want;
+  return GMOE_OK;
+}
+
+// Counters of n groups' parts a kv head.
+gmoe_status grow_done(gmoe_kv* kv, size_t n) {
+  n *= kv->d.n_kv_heads;
+  if (n <= kv->n_done) return GMOE_OK;
+  KV_TRY(hipDeviceSynchronize());  // queued calls may still use the old ones
+  if (kv->done) KV_TRY(hipFree(kv->done));
+  kv->done = nullptr;
+  kv->n_done = 0;
+  kv->scratch_id++;
+  const size_t want = std::max(n, (size_t)4096);
+  KV_TRY(hipMalloc((void**)&kv->done, want * sizeof(uint32_t)));
+  KV_TRY(hipMemset(kv->done, 0, want * sizeof(uint32_t)));
+  KV_TRY(hipDeviceSynchronize());  // before a call on any stream
+  kv->n_done = want;
   return GMOE_OK;
 }
 
@@ -329,6 +351,7 @@ Kv8Args args8(const gmoe_kv* kv, uint32_t n, const float* q, const float* k, con
   a.ctx = out;
   a.q_stride = q_stride ? q_stride : D.n_heads * D.head_dim;
   a.kv_stride = kv_stride ? kv_stride : kv->kvd;
+  a.done = kv->done;
   return a;
 }
 
@@ -417,6 +440,18 @@ void job_pages(std::vector<Kv8Job>& jobs, const AttnEntry* ent) {
   }
 }
 
+// Whether a step's workgroups may write its context while others have yet to read: it lies
+// apart from the inputs, or is the queries' own rows, which only a row's own workgroups read.
+bool apart(const Kv8Args& a) {
+  const size_t n = a.n, qd = (size_t)a.n_heads * a.p.hd, kvd = (size_t)a.p.n_kv * a.p.hd;
+  auto over = [&](const float* p, size_t width, size_t stride) {
+    const uintptr_t c = (uintptr_t)a.ctx, i = (uintptr_t)p;
+    return c < i + ((n - 1) * stride + width) * 4 && i < c + n * qd * 4;
+  };
+  if (over(a.k, kvd, a.kv_stride) || over(a.v, kvd, a.kv_stride)) return false;
+  return !over(a.q, qd, a.q_stride) || (a.ctx == a.q && a.q_stride == qd);
+}
+
 // attend() for a cache in 8 bits; with `out` null the tokens are only appended.
 gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* q, const float* k,
                     const float* v, float* out, hipStream_t st, uint32_t q_stride, uint32_t kv_stride) {
@@ -425,13 +460,16 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   uint32_t maxspan;
   bool distinct;
   if (gmoe_status s = plan(kv, layer, seqs, n, ent.data(), &maxspan, &distinct)) return s;
+  if (out)
+    if (gmoe_status s = grow_done(kv, n)) return s;  // a group is of a token at least
   Kv8Args a = args8(kv, n, q, k, v, out, q_stride, kv_stride);
   uint8_t* pin = nullptr;
-  if (out && distinct) {
+  if (out && distinct && apart(a)) {
     Kv8Inline inl{};
     const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
     a.nparts = kv8_parts(maxspan);
     for (uint32_t i = 0; i < n; i++) a.items += kv8_parts_of(ent[i].pos, ent[i].start);
+    a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv->d.n_heads / kv->d.n_kv_heads * kv->d.head_dim);
     if (gmoe_status s = grow_scratch(kv, eb + step8_bytes(kv, n, a.nparts))) return s;
     if (eb)
       if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
@@ -458,6 +496,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   };
   size_t o_run = 0, o_qr = 0, o_own = 0, o_max = 0, o_part = 0, o_tpart = 0;
   if (out) {
+    const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
     cut_runs(kv, runs, groups, tiles);
     a.nrun = (uint32_t)groups.size();
     a.ntile = (uint32_t)tiles.size();
@@ -466,8 +505,9 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
       uint32_t span = 1;  // a group's first token has the longest way back of its tokens, or as long a one
       for (const Kv8Run& g : groups) span = std::max(span, ent[g.i0 + g.n - 1].pos + 1 - ent[g.i0].start);
       a.nparts = kv8_parts(span);
+      for (const Kv8Run& g : groups) a.items += kv8_parts_of(g.pos0, ent[g.i0].start);
+      a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv8_group_tokens(G) * G * kv->d.head_dim);
     }
-    const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
     o_run = take((groups.size() + tiles.size()) * sizeof(Kv8Run));
     o_qr = take((size_t)n * kv->d.n_heads * kv->d.head_dim * 4);
     o_own = take(jobs.size() * 2 * kKv8Block * kv->kvd * 4);
@@ -837,10 +877,12 @@ gmoe_status kv_reserve(gmoe_kv* kv, uint32_t n, uint32_t nchunk) {
     return kfail(GMOE_ERR_DEVICE, "attention scratch of %zu bytes: allocation refused (test hook)",
                  step_bytes(kv, n, nchunk));
   }
+  if (kv->q8)
+    if (gmoe_status s = grow_done(kv, n)) return s;
   return grow_scratch(kv, step_bytes(kv, n, nchunk));
 }
 
-const void* kv_scratch_id(gmoe_kv* kv) { return kv->scratch; }
+const void* kv_scratch_id(gmoe_kv* kv) { return (const void*)kv->scratch_id; }
 
 gmoe_status kv_plan_commit(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, AttnEntry* ent) {
   std::lock_guard<std::mutex> g(kv->mu);
@@ -863,7 +905,8 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
     a.part = reinterpret_cast<float*>(kv->scratch);
     a.nparts = kv8_parts(nchunk * kAttnChunk);
     a.items = n * a.nparts;
-    if (step_bytes(kv, n, nchunk) > kv->scratch_bytes) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
+    a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv->d.n_heads / kv->d.n_kv_heads * kv->d.head_dim);
+    if (step_bytes(kv, n, nchunk) > kv->scratch_bytes || (size_t)n * kv->d.n_kv_heads > kv->n_done) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
     KV_TRY(launch_kv8_step(a, Kv8Inline{}, st));
     return GMOE_OK;
   }
