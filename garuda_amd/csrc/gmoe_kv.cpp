@@ -355,55 +355,113 @@ Kv8Args args8(const gmoe_kv* kv, uint32_t n, const float* q, const float* k, con
   return a;
 }
 
-// The blocks that a planned call appends to, those of one sequence in position order (pages:
-// job_pages, after the commit), and its runs: consecutive entries of one sequence.
-void find_jobs(const gmoe_kv* kv, const uint32_t* seqs, uint32_t n, const AttnEntry* ent, std::vector<Kv8Job>& jobs,
-               std::vector<Kv8Run>& runs) {
+// A call on a cache in 8 bits: its runs (consecutive entries of one sequence; job not yet
+// known), and of each sequence its tokens in the call, its first position and its first block's
+// job. Checked against the window and the free pages as plan() checks entries, run by run.
+struct Plan8 {
   struct Of {
     uint32_t count = 0, pos0 = 0, job = 0;
   };
-  std::vector<Of> of(kv->seqs.size());
+  std::vector<Kv8Run> runs;
+  std::vector<uint32_t> seq;  // [run]
+  std::vector<Of> of;         // [sequence]
+  uint32_t njob = 0;
+  bool distinct = true;       // no sequence has two entries
+};
+gmoe_status plan8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, Plan8& P) {
+  const gmoe_kv_desc& D = kv->d;
+  if (layer >= D.n_layers) return kfail(GMOE_ERR_INFERENCE, "layer %u of %u", layer, D.n_layers);
+  if (n == 0 || !seqs) return kfail(GMOE_ERR_INFERENCE, "empty attention call");
+  P.of.resize(kv->seqs.size());
   for (uint32_t i = 0; i < n; i++) {
-    Of& o = of[seqs[i]];
-    if (!o.count++) o.pos0 = ent[i].pos;
-  }
-  for (uint32_t i = 0; i < n; i++) {
-    Of& o = of[seqs[i]];
-    const uint32_t block = ent[i].pos / kKv8Block, row = ent[i].pos % kKv8Block;
-    const uint32_t table = (uint32_t)((ent[i].pages - kv->tables) / kv->ppseq);
-    if (ent[i].pos == o.pos0) {
-      o.job = (uint32_t)jobs.size();
-      const uint32_t nb = (o.pos0 % kKv8Block + o.count + kKv8Block - 1) / kKv8Block;
-      for (uint32_t b = 0; b < nb; b++) {
-        Kv8Job j{};
-        j.table = table;
-        j.block = block + b;
-        j.r0 = b ? 0 : row;
-        j.n = std::min(kKv8Block - j.r0, o.pos0 + o.count - (j.block * kKv8Block + j.r0));
-        j.flags = (b ? 0 : kKv8First) | (j.r0 + j.n == kKv8Block ? kKv8Whole : 0);
-        j.last = o.job + nb - 1;
-        jobs.push_back(j);
-      }
+    if (i && seqs[i] == seqs[i - 1]) {
+      P.runs.back().n++;
+      continue;
     }
-    const uint32_t job = o.job + block - o.pos0 / kKv8Block;
-    jobs[job].ent[row] = i;
-    if (i && ent[i - 1].pages == ent[i].pages) runs.back().n++;
-    else runs.push_back(Kv8Run{i, 1, ent[i].pos, job, table});
+    const uint32_t s = seqs[i];
+    if (s >= kv->seqs.size() || !kv->seqs[s].open) return kfail(GMOE_ERR_INFERENCE, "sequence %u is not open", s);
+    P.runs.push_back(Kv8Run{i, 1, 0, 0, s * D.n_layers + layer});
+    P.seq.push_back(s);
+  }
+  uint64_t need = 0;
+  for (size_t r = 0; r < P.runs.size(); r++) {
+    Plan8::Of& o = P.of[P.seq[r]];
+    Kv8Run& R = P.runs[r];
+    if (!o.count) o.pos0 = kv->seqs[P.seq[r]].len[layer];
+    R.pos0 = o.pos0 + o.count;
+    const uint64_t end = (uint64_t)R.pos0 + R.n;
+    if (end > D.max_positions) return kfail(GMOE_ERR_CACHE, "context window of %u positions is exhausted", D.max_positions);
+    need += (end + D.block_size - 1) / D.block_size - ((uint64_t)R.pos0 + D.block_size - 1) / D.block_size;
+    const uint32_t before = o.count ? (o.pos0 % kKv8Block + o.count + kKv8Block - 1) / kKv8Block : 0;
+    o.count += R.n;
+    P.njob += (o.pos0 % kKv8Block + o.count + kKv8Block - 1) / kKv8Block - before;
+    P.distinct &= o.count == 1;
+  }
+  if (need > kv->free_pages.size())
+    return kfail(GMOE_ERR_CACHE, "the KV pool has %zu free pages, the call needs %llu", kv->free_pages.size(),
+                 (unsigned long long)need);
+  return GMOE_OK;
+}
+
+// Commits a planned call: lengths advance and pages are taken.
+void commit8(gmoe_kv* kv, uint32_t layer, const Plan8& P) {
+  for (size_t r = 0; r < P.runs.size(); r++) {
+    Seq& S = kv->seqs[P.seq[r]];
+    const uint32_t end = P.runs[r].pos0 + P.runs[r].n;
+    while ((uint64_t)S.pages[layer].size() * kv->d.block_size < end) {
+      S.pages[layer].push_back(kv->free_pages.back());
+      kv->free_pages.pop_back();
+    }
+    S.len[layer] = end;
+    S.open_block[layer] = (end - 1) / kKv8Block;
   }
 }
 
-// The runs cut into groups of at most 16 rows, or tiles of at most 256 where a run has rows for
+// The blocks that a committed call appends to, those of one sequence in position order.
+void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
+  const uint32_t bs = kv->d.block_size;
+  uint32_t nj = 0;
+  for (size_t r = 0; r < P.runs.size(); r++) {
+    Plan8::Of& o = P.of[P.seq[r]];
+    Kv8Run& R = P.runs[r];
+    const uint32_t b0 = o.pos0 / kKv8Block, end = o.pos0 + o.count, nb = (end + kKv8Block - 1) / kKv8Block - b0;
+    if (R.pos0 == o.pos0) {
+      const std::vector<uint32_t>& pages = kv->seqs[P.seq[r]].pages[layer];
+      o.job = nj;
+      for (uint32_t b = 0; b < nb; b++) {
+        Kv8Job& j = jobs[nj++];
+        j = Kv8Job{};
+        j.table = R.table;
+        j.block = b0 + b;
+        j.page = pages[j.block * kKv8Block / bs];
+        j.r0 = b ? 0 : o.pos0 % kKv8Block;
+        j.n = std::min(kKv8Block - j.r0, end - (j.block * kKv8Block + j.r0));
+        j.flags = (b ? 0 : kKv8First) | (j.r0 + j.n == kKv8Block ? kKv8Whole : 0) |
+                  (j.r0 == 0 && j.block * kKv8Block % bs == 0 ? kKv8Fresh : 0);
+        j.last = o.job + nb - 1;
+      }
+    }
+    R.job = o.job + R.pos0 / kKv8Block - b0;
+    for (uint32_t t = 0; t < R.n; t++) {
+      const uint32_t pos = R.pos0 + t;
+      jobs[o.job + pos / kKv8Block - b0].ent[pos % kKv8Block] = R.i0 + t;
+    }
+  }
+}
+
+// The runs cut into groups (job: the run's index, for now) of at most 16 rows, or tiles of at most 256 where a run has rows for
 // a quarter of one: with fewer, most of a tile's waves idle while the groups read the cache
 // a few times.
 constexpr uint32_t kKv8TileMin = 64;
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
   const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
-  for (const Kv8Run& r : runs) {
+  for (uint32_t i = 0; i < runs.size(); i++) {
+    const Kv8Run& r = runs[i];
     const bool tile = kv->d.head_dim <= kKv8TileHd && (uint64_t)r.n * G >= kKv8TileMin;
     for (uint32_t at = 0, m; at < r.n; at += m) {
       const uint32_t pos = r.pos0 + at;
       m = std::min(r.n - at, tile ? kv8_tile_tokens(G) : std::min(kv8_group_tokens(G), kKv8Block - pos % kKv8Block));
-      (tile ? tiles : groups).push_back(Kv8Run{r.i0 + at, m, pos, r.job + pos / kKv8Block - r.pos0 / kKv8Block, r.table});
+      (tile ? tiles : groups).push_back(Kv8Run{r.i0 + at, m, pos, i, r.table});
     }
   }
 }
@@ -432,14 +490,6 @@ size_t step8_bytes(const gmoe_kv* kv, uint32_t n, uint32_t nparts) {
   return part8_bytes(kv, n, kv->d.n_heads / kv->d.n_kv_heads, nparts);
 }
 
-void job_pages(std::vector<Kv8Job>& jobs, const AttnEntry* ent) {
-  for (Kv8Job& j : jobs) {
-    const AttnEntry& e = ent[j.ent[j.r0]];
-    j.page = e.page;
-    if (e.fresh) j.flags |= kKv8Fresh;  // a page opens with a block
-  }
-}
-
 // Whether a step's workgroups may write its context while others have yet to read: it lies
 // apart from the inputs, or is the queries' own rows, which only a row's own workgroups read.
 bool apart(const Kv8Args& a) {
@@ -456,38 +506,44 @@ bool apart(const Kv8Args& a) {
 gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* q, const float* k,
                     const float* v, float* out, hipStream_t st, uint32_t q_stride, uint32_t kv_stride) {
   if (gmoe_status s = refuse_capture(st)) return s;
-  std::vector<AttnEntry> ent(n ? n : 1);
-  uint32_t maxspan;
-  bool distinct;
-  if (gmoe_status s = plan(kv, layer, seqs, n, ent.data(), &maxspan, &distinct)) return s;
+  Plan8 P;
+  if (gmoe_status s = plan8(kv, layer, seqs, n, P)) return s;
   if (out)
     if (gmoe_status s = grow_done(kv, n)) return s;  // a group is of a token at least
   Kv8Args a = args8(kv, n, q, k, v, out, q_stride, kv_stride);
+  const gmoe_kv_desc& D = kv->d;
+  const uint32_t G = D.n_heads / D.n_kv_heads;
+  auto start_of = [&](uint32_t pos) { return D.sliding_window && pos + 1 > D.sliding_window ? pos + 1 - D.sliding_window : 0; };
   uint8_t* pin = nullptr;
-  if (out && distinct && apart(a)) {
-    Kv8Inline inl{};
+  if (out && P.distinct && apart(a)) {
+    uint32_t span = 1;
+    for (const Kv8Run& r : P.runs) {
+      span = std::max(span, r.pos0 + 1 - start_of(r.pos0));
+      a.items += kv8_parts_of(r.pos0, start_of(r.pos0));
+    }
+    a.nparts = kv8_parts(span);
+    a.fused = kv8_fused(a.items, D.n_kv_heads, a.nparts, G * D.head_dim);
     const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
-    a.nparts = kv8_parts(maxspan);
-    for (uint32_t i = 0; i < n; i++) a.items += kv8_parts_of(ent[i].pos, ent[i].start);
-    a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv->d.n_heads / kv->d.n_kv_heads * kv->d.head_dim);
     if (gmoe_status s = grow_scratch(kv, eb + step8_bytes(kv, n, a.nparts))) return s;
     if (eb)
       if (gmoe_status s = take_pinned(kv, eb, st, &pin)) return s;
     a.part = reinterpret_cast<float*>(kv->scratch + eb);
-    commit(kv, layer, seqs, n, ent.data());
+    commit8(kv, layer, P);
+    Kv8Inline inl;
+    AttnEntry* ent = pin ? reinterpret_cast<AttnEntry*>(pin) : inl.e;
+    for (uint32_t i = 0; i < n; i++) {
+      const uint32_t pos = P.runs[i].pos0;
+      ent[i] = AttnEntry{kv->tables + (size_t)P.runs[i].table * kv->ppseq, pos, start_of(pos),
+                         kv->seqs[P.seq[i]].pages[layer][pos / D.block_size], pos % D.block_size == 0 ? 1u : 0u};
+    }
     if (pin) {
-      memcpy(pin, ent.data(), n * sizeof(AttnEntry));
       KV_TRY(hipMemcpyAsync(kv->scratch, pin, n * sizeof(AttnEntry), hipMemcpyHostToDevice, st));
       a.ent = reinterpret_cast<const AttnEntry*>(kv->scratch);
-    } else {
-      std::copy(ent.begin(), ent.begin() + n, inl.e);
     }
     KV_TRY(launch_kv8_step(a, inl, st));
     return GMOE_OK;
   }
-  std::vector<Kv8Job> jobs;
-  std::vector<Kv8Run> runs, groups, tiles;
-  find_jobs(kv, seqs, n, ent.data(), jobs, runs);
+  std::vector<Kv8Run> groups, tiles;
   size_t at = 0;
   auto take = [&](size_t bytes) {  // of the scratch
     const size_t o = at;
@@ -496,36 +552,42 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
   };
   size_t o_run = 0, o_qr = 0, o_own = 0, o_max = 0, o_part = 0, o_tpart = 0;
   if (out) {
-    const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
-    cut_runs(kv, runs, groups, tiles);
+    cut_runs(kv, P.runs, groups, tiles);
     a.nrun = (uint32_t)groups.size();
     a.ntile = (uint32_t)tiles.size();
     if (a.ntile) a.tkeys = tile_split(kv, tiles, &a.tsplits);
     if (a.nrun) {
-      uint32_t span = 1;  // a group's first token has the longest way back of its tokens, or as long a one
-      for (const Kv8Run& g : groups) span = std::max(span, ent[g.i0 + g.n - 1].pos + 1 - ent[g.i0].start);
+      uint32_t span = 1;
+      for (const Kv8Run& g : groups) {
+        span = std::max(span, g.pos0 + g.n - start_of(g.pos0));
+        a.items += kv8_parts_of(g.pos0, start_of(g.pos0));
+      }
       a.nparts = kv8_parts(span);
-      for (const Kv8Run& g : groups) a.items += kv8_parts_of(g.pos0, ent[g.i0].start);
-      a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv8_group_tokens(G) * G * kv->d.head_dim);
+      a.fused = kv8_fused(a.items, D.n_kv_heads, a.nparts, kv8_group_tokens(G) * G * D.head_dim);
     }
     o_run = take((groups.size() + tiles.size()) * sizeof(Kv8Run));
-    o_qr = take((size_t)n * kv->d.n_heads * kv->d.head_dim * 4);
-    o_own = take(jobs.size() * 2 * kKv8Block * kv->kvd * 4);
-    o_max = take(jobs.size() * kv->d.n_kv_heads * sizeof(float2));
+    o_qr = take((size_t)n * D.n_heads * D.head_dim * 4);
+    o_own = take((size_t)P.njob * 2 * kKv8Block * kv->kvd * 4);
+    o_max = take((size_t)P.njob * D.n_kv_heads * sizeof(float2));
     o_part = take(part8_bytes(kv, groups.size(), kv8_group_tokens(G) * G, a.nparts));
     o_tpart = take(part8_bytes(kv, tiles.size(), kKv8TileRows, a.tsplits));
     if (gmoe_status s = grow_scratch(kv, at)) return s;
   }
-  const size_t jb = jobs.size() * sizeof(Kv8Job), gb = groups.size() * sizeof(Kv8Run), tb = tiles.size() * sizeof(Kv8Run);
-  if (gmoe_status s = take_pinned(kv, jb + gb + tb, st, &pin)) return s;
-  commit(kv, layer, seqs, n, ent.data());
-  job_pages(jobs, ent.data());
-  memcpy(pin, jobs.data(), jb);
-  if (gb) memcpy(pin + jb, groups.data(), gb);
-  if (tb) memcpy(pin + jb + gb, tiles.data(), tb);
-  a.hjob = reinterpret_cast<const Kv8Job*>(pin);
+  const size_t jb = P.njob * sizeof(Kv8Job), rb = (groups.size() + tiles.size()) * sizeof(Kv8Run);
+  if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
+  commit8(kv, layer, P);
+  Kv8Job* jobs = reinterpret_cast<Kv8Job*>(pin);
+  fill_jobs(kv, layer, P, jobs);
+  Kv8Run* runs = reinterpret_cast<Kv8Run*>(pin + jb);
+  for (const std::vector<Kv8Run>* v : {&groups, &tiles})
+    for (Kv8Run r : *v) {  // a piece of run r.job
+      const Kv8Run& of = P.runs[r.job];
+      r.job = of.job + r.pos0 / kKv8Block - of.pos0 / kKv8Block;
+      *runs++ = r;
+    }
+  a.hjob = jobs;
   a.hrun = reinterpret_cast<const Kv8Run*>(pin + jb);
-  a.njob = (uint32_t)jobs.size();
+  a.njob = P.njob;
   if (out) {
     a.run = reinterpret_cast<Kv8Run*>(kv->scratch + o_run);
     a.qr = reinterpret_cast<float*>(kv->scratch + o_qr);
@@ -571,20 +633,19 @@ gmoe_status read_rows(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const u
   if (gmoe_status s = refuse_capture(st)) return s;
   std::vector<Kv8Rows> rows;
   const uint32_t per = kv->q8 ? kKv8Block : D.block_size;
+  uint32_t more = 0;  // positions that the last piece may still take: up to its end, or the sequence's
   for (uint32_t i = 0; i < n; i++) {
     const uint32_t s = seqs[i];
+    if (more && s == seqs[i - 1] && pos[i] == pos[i - 1] + 1) {
+      rows.back().n++;
+      more--;
+      continue;
+    }
     if (s >= kv->seqs.size() || !kv->seqs[s].open) return kfail(GMOE_ERR_INFERENCE, "sequence %u is not open", s);
     const uint32_t len = kv->seqs[s].len[layer], b = pos[i] / per, r = pos[i] % per;
     if (pos[i] >= len) return kfail(GMOE_ERR_INFERENCE, "position %u of a sequence of %u", pos[i], len);
-    const uint32_t table = s * D.n_layers + layer;
-    if (!rows.empty()) {
-      Kv8Rows& l = rows.back();
-      if (l.table == table && l.block == b && l.r0 + l.n == r && l.n < kKv8Block) {
-        l.n++;
-        continue;
-      }
-    }
-    rows.push_back(Kv8Rows{table, b, i, r, 1, kv->q8 && (uint64_t)(b + 1) * kKv8Block <= len});
+    rows.push_back(Kv8Rows{s * D.n_layers + layer, b, i, r, 1, kv->q8 && (uint64_t)(b + 1) * kKv8Block <= len});
+    more = std::min(std::min(per - r, kKv8Block), len - pos[i]) - 1;
   }
   Kv8RowsInline inl{};
   uint8_t* pin = nullptr;
