@@ -1103,7 +1103,7 @@ __device__ __forceinline__ void rows_again(const Kv8Args& a, const Kv8Run& run, 
 // 16 scores of 32 positions are 8 consecutive ones of each of two blocks, its own half of
 // the second product's B operand; O^T = V^T P^T.
 //
-// Split 0 then takes the rows' own blocks, 32 positions at a time: f32 rows, scaled by a power of
+// Split 0 takes the rows' own blocks after its positions, or by itself, 32 positions at a time: f32 rows, scaled by a power of
 // two for each block, as two fp16 each, three of the four products of two such sums (the
 // fourth is 2^-22 of the first). A row that meets a score that is NaN or +inf, or whose own block
 // has a value that is not finite, is marked and summed again by itself in f32 (row_again).
@@ -1136,6 +1136,9 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   __shared__ uint32_t marks[8];  // rows to be summed again, a bit each
   const Kv8Pool& p = a.p;
   const uint32_t h = blockIdx.x, x = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
+  // the own blocks by split 0, or by one of their own before the others
+  const bool owns = z == 0;
+  const uint32_t zk = z - a.town;
   const uint32_t lane = t & 63, l32 = lane & 31, hf = lane >> 5;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
   auto uni = [](uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane(v); };
@@ -1144,13 +1147,13 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   const uint32_t rows = ntok * G, last = pos0 + ntok - 1;
   auto start_of = [&](uint32_t pos) { return kv8_start(a, pos); };
   auto own_of = [](uint32_t pos) { return pos / kKv8Block * kKv8Block; };
-  const uint32_t base = own_of(start_of(pos0)), lo = base + z * a.tkeys, hi = min(own_of(last), lo + a.tkeys);
+  const uint32_t base = own_of(start_of(pos0)), lo = base + zk * a.tkeys, hi = a.town && owns ? 0 : min(own_of(last), lo + a.tkeys);
   const uint32_t row = 32 * wave + l32, rr = min(row, rows - 1), pos = pos0 + rr / G;
   const uint32_t start = start_of(pos), own = own_of(pos);
   const Kv8Part part = tile_parts(a);
   const size_t prow = part.row(z, x, h, row);  // 256 rows a kv head
   const bool mine = row < rows, busy = 32 * wave < rows;
-  if (z && lo >= hi) return;
+  if (!owns && lo >= hi) return;
   // what the wave's rows attend to of the held blocks: from its first row's start to its last row's own block
   const uint32_t pw0 = pos0 + min(32 * wave, rows - 1) / G, pw1 = pos0 + min(32 * wave + 31, rows - 1) / G;
   const uint32_t w_lo = start_of(pw0), w_hi = min(own_of(pw1), hi), w_in0 = start_of(pw1), w_in1 = min(own_of(pw0), hi);
@@ -1191,7 +1194,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     *reinterpret_cast<f16x8*>(buf + KB + sx * 128 + (((2 * sb + 1) ^ (sx % 8)) * 16)) = codes8(vc.z, vc.w);
     if (sx == 0) sc[b][sb] = sv2;
   };
-  const bool any = lo < hi;
+  const bool any = !(a.town && owns) && lo < hi;
   size_t unit = 0;
   if (any) {
     unit = find(lo);
@@ -1354,7 +1357,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   if (any) store(0);
   __syncthreads();
   uint32_t buf = 0;
-  for (uint32_t kb = lo; kb < hi; kb += 64, buf ^= 1) {
+  for (uint32_t kb = lo; any && kb < hi; kb += 64, buf ^= 1) {
     const bool more = kb + 64 < hi;
     if (more) {
       load(unit);
@@ -1366,7 +1369,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
     if (more) store(buf ^ 1);
     __syncthreads();
   }
-  if (z == 0) {
+  if (owns) {
     // the rows' own blocks, two at a time: planes of keys [2][32][HDP], of values transposed [2][HDP][32]
     constexpr uint32_t PK = 32 * HDP * 2, PV = HDP * 32 * 2;
     const uint32_t b_end = last / kKv8Block;
@@ -1522,7 +1525,8 @@ __global__ void __launch_bounds__(256) k8_join_tile(Kv8Args a) {
   __syncthreads();
   if (t / q4 < rpw && r < rows) {
     const uint32_t last = run.pos0 + run.n - 1, first = kv8_start(a, run.pos0);
-    const uint32_t n = max(1u, (last / kKv8Block * kKv8Block - first / kKv8Block * kKv8Block + a.tkeys - 1) / a.tkeys);
+    const uint32_t held = (last / kKv8Block * kKv8Block - first / kKv8Block * kKv8Block + a.tkeys - 1) / a.tkeys;
+    const uint32_t n = max(1u, a.town + held);
     Joined j;
     j.parts<false, 2>(part, 0, n, part.row(0, x, h, r), hd, c);
     float4 v;

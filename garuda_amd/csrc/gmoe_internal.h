@@ -550,8 +550,8 @@ struct Kv8Args {
   uint32_t* done;      // [groups][n_kv] parts that are written; 0 between calls
   uint32_t fused;      // 1: the last workgroup of a group joins its parts (kv8_fused)
   uint32_t items;      // the groups' parts, over all entries
-  float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions
-  uint32_t tsplits, tkeys;
+  float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions, the first of them
+  uint32_t tsplits, tkeys, town;  // the rows' own blocks alone where town is 1
 };
 struct Kv8Inline {
   AttnEntry e[kKv8Inline];

@@ -469,7 +469,7 @@ void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv
 // Positions of a tile's split: the tiles' keys are split over workgroups until the call has
 // about one a CU, each split keeping at least four steps of 64 positions.
 constexpr uint32_t kKv8TileWgs = 256;
-uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_t* splits) {
+uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_t* splits, uint32_t* own) {
   uint32_t span = 1;
   for (const Kv8Run& t : tiles) {
     const uint32_t w = kv->d.sliding_window, from = w && t.pos0 + 1 > w ? t.pos0 + 1 - w : 0;
@@ -479,6 +479,10 @@ uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_
   const uint32_t ns = std::max(1u, std::min((kKv8TileWgs + wgs - 1) / wgs, steps / 4));
   const uint32_t keys = (steps + ns - 1) / ns * 64;
   *splits = (span + keys - 1) / keys;
+  // the own blocks in a split of their own where there are CUs for it: a split of few positions took
+  // as long again for them
+  *own = *splits > 1 && wgs * (*splits + 1) <= kKv8TileWgs ? 1 : 0;
+  *splits += *own;
   return keys;
 }
 
@@ -555,7 +559,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     cut_runs(kv, P.runs, groups, tiles);
     a.nrun = (uint32_t)groups.size();
     a.ntile = (uint32_t)tiles.size();
-    if (a.ntile) a.tkeys = tile_split(kv, tiles, &a.tsplits);
+    if (a.ntile) a.tkeys = tile_split(kv, tiles, &a.tsplits, &a.town);
     if (a.nrun) {
       uint32_t span = 1;
       for (const Kv8Run& g : groups) {
