@@ -449,18 +449,29 @@ void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
   }
 }
 
-// The runs cut into groups (job: the run's index, for now) of at most 16 rows, or tiles of at most 256 where a run has rows for
-// a quarter of one: with fewer, most of a tile's waves idle while the groups read the cache
-// a few times.
-constexpr uint32_t kKv8TileMin = 64;
+// The runs cut into groups (job: the run's index, for now) of at most 16 rows, or into tiles of
+// at most 256. A group reads the cache for itself, but a call of few groups has them all on the
+// card at once, where a tile's waves without rows idle; so runs of 48 rows or more go in tiles
+// where as groups they would make more workgroups than two a CU twice over. 32 heads on 8 of
+// 128, in groups and in tiles: 32 tokens at 3008 (448 workgroups) 31 and 36 us, at 12000 (1600)
+// 53 and 49; 16 tokens of each of 6 sequences at 3008 (1344) 55.5 and 53.7, 32 of each 88 and
+// 58; 12 of each (1008) 46 and 52. 64 tokens at 2000, 8 heads on 2 of 32 (160): 19.5 and 27.
+constexpr uint32_t kKv8TileMin = 48, kKv8GroupWgs = 1024;
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
-  const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads;
+  const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads, T = kv8_group_tokens(G), w = kv->d.sliding_window;
+  auto large = [&](const Kv8Run& r) { return kv->d.head_dim <= kKv8TileHd && (uint64_t)r.n * G >= kKv8TileMin; };
+  uint64_t wgs = 0;
+  for (const Kv8Run& r : runs)
+    if (large(r)) {
+      const uint32_t end = r.pos0 + r.n - 1;
+      wgs += (uint64_t)((r.n + T - 1) / T) * kv8_parts_of(end, w && end + 1 > w ? end + 1 - w : 0) * kv->d.n_kv_heads;
+    }
   for (uint32_t i = 0; i < runs.size(); i++) {
     const Kv8Run& r = runs[i];
-    const bool tile = kv->d.head_dim <= kKv8TileHd && (uint64_t)r.n * G >= kKv8TileMin;
+    const bool tile = wgs > kKv8GroupWgs && large(r);
     for (uint32_t at = 0, m; at < r.n; at += m) {
       const uint32_t pos = r.pos0 + at;
-      m = std::min(r.n - at, tile ? kv8_tile_tokens(G) : std::min(kv8_group_tokens(G), kKv8Block - pos % kKv8Block));
+      m = std::min(r.n - at, tile ? kv8_tile_tokens(G) : std::min(T, kKv8Block - pos % kKv8Block));
       (tile ? tiles : groups).push_back(Kv8Run{r.i0 + at, m, pos, i, r.table});
     }
   }
