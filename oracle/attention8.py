@@ -105,17 +105,64 @@ class Kv8Oracle:
         return out.reshape(-1), mag
 
     def append(self, layer, seqs, k, v):
-        return [self.append_one(layer, int(s), k[i], v[i]) for i, s in enumerate(seqs)]
+        """Entries in order; returns their positions."""
+        seqs = [int(s) for s in seqs]
+        at, pos = 0, []
+        while at < len(seqs):
+            n = at + 1
+            while n < len(seqs) and seqs[n] == seqs[at]:
+                n += 1
+            pos += self._append_run(layer, seqs[at], k[at:n], v[at:n])
+            at = n
+        return pos
+
+    def _append_run(self, layer, seq, k, v):
+        r = self.of(seq, layer)
+        p0, n = len(r.given[0]), len(k)
+        if p0 + n > self.maxpos:
+            raise ValueError("context window exhausted")
+        k = np.asarray(k, np.float32).reshape(n, self.nkv, self.hd)
+        new = (np.stack([rope64(k[i], p0 + i, self.theta) for i in range(n)]),
+               np.asarray(v, np.float32).reshape(n, self.nkv, self.hd))
+        for j in range(2):
+            r.given[j] = np.concatenate([r.given[j], new[j]])
+            done = range(len(r.held[j]), (p0 + n) // BLOCK * BLOCK, BLOCK)
+            r.held[j] = np.concatenate([r.held[j], *(hold(r.given[j][b:b + BLOCK]) for b in done)])
+        r.open_block = (p0 + n - 1) // BLOCK
+        return list(range(p0, p0 + n))
 
     def attention(self, layer, seqs, q, k, v):
         """Entries in order: contexts [n, nh * hd], and the bound of attend_one over all."""
+        pos = self.append(layer, seqs, k, v)
         out, mag = [], 0.0
         for i, s in enumerate(seqs):
-            pos = self.append_one(layer, int(s), k[i], v[i])
-            c, m = self.attend_one(layer, int(s), pos, q[i])
+            c, m = self.attend_one(layer, int(s), pos[i], q[i])
             out.append(c)
             mag = max(mag, m)
         return np.stack(out), mag
+
+    def attend_run(self, layer, seq, pos0, q):
+        """attend_one of consecutive positions from pos0 on, all input finite and its scores within f32."""
+        n, g, r = len(q), self.nh // self.nkv, self.of(seq, layer)
+        q = np.stack([rope64(np.asarray(q[i], np.float32).reshape(self.nh, self.hd), pos0 + i, self.theta)
+                      for i in range(n)]).astype(np.float64)
+        end = pos0 + n
+        at, key = np.arange(pos0, end)[:, None], np.arange(end)[None]
+        near, seen = key // BLOCK == at // BLOCK, key <= at
+        if self.win:
+            seen &= key > at - self.win
+        given = [x[:end].astype(np.float64) for x in r.given]
+        held = [np.concatenate([h[:end], g_[len(h):end]]).astype(np.float64) for h, g_ in zip(r.held, r.given)]
+        out, mag = np.empty((n, self.nh, self.hd)), 0.0
+        for h in range(self.nh):
+            kg, kh, vg, vh = given[0][:, h // g], held[0][:, h // g], given[1][:, h // g], held[1][:, h // g]
+            s = np.where(near, q[:, h] @ kg.T, q[:, h] @ kh.T) / np.sqrt(self.hd)
+            s = np.where(seen, s, -np.inf)
+            w = np.exp(s - s.max(1, keepdims=True))
+            w /= w.sum(1, keepdims=True)
+            out[:, h] = (w * near) @ vg + (w * ~near) @ vh
+            mag = max(mag, float((np.abs(q[:, h]) @ np.abs(kg).T).max() / np.sqrt(self.hd)))
+        return out.reshape(n, -1), mag
 
     def read(self, layer, seqs, positions):
         out = [[], []]

@@ -60,6 +60,24 @@ def test_equal_values_come_back_and_truncation_reopens():
     assert o.seq_len(0) == 16 and len(o.of(0, 0).held[0]) == 16
 
 
+@pytest.mark.parametrize("window", [0, 30])
+def test_runs_are_the_tokens_one_by_one(window):
+    nh, nkv, hd = 4, 2, 16
+    rng = np.random.default_rng(4)
+    a, b = (Kv8Oracle(1, nh, nkv, hd, sliding_window=window) for _ in range(2))
+    at = 0
+    for n in (21, 1, 50, 9):
+        q, k, v = (rng.normal(size=(n, w * hd)).astype(np.float32) for w in (nh, nkv, nkv))
+        one, _ = a.attention(0, [0] * n, q, k, v)
+        for i in range(n):
+            assert b.append_one(0, 0, k[i], v[i]) == at + i
+        run, _ = b.attend_run(0, 0, at, q)
+        assert np.allclose(run, one, rtol=1e-12, atol=1e-12)
+        at += n
+    for x, y in zip(a.read(0, [0] * at, range(at)), b.read(0, [0] * at, range(at))):
+        assert np.array_equal(x, y)
+
+
 def test_null_arguments_are_refused_without_a_device():
     lib = _lib.lib()
     x = np.zeros(4, np.float32)

@@ -126,6 +126,45 @@ def test_steps_and_prompts_of_every_head_layout(dev, nh, nkv, hd):
         assert kv.seq_len(seqs[0], 0) == 0
 
 
+def workgroups(nh, nkv, spans):
+    """Groups of 16 rows and splits of their spans that a call of runs (start, end) would make: above 1024 of
+    them, runs of 48 rows and more go in tiles."""
+    g = nh // nkv
+    return sum(-(-(e - s) // (16 // g)) * (1 + -(-((e - 1) // BLOCK * BLOCK) // 512)) * nkv for s, e in spans)
+
+
+@pytest.mark.parametrize("nh,nkv,hd,bs,window,sizes", [
+    (8, 2, 64, 16, 0, [300] * 8), (32, 8, 128, 16, 0, [150, 400]), (4, 4, 32, 32, 0, [520] * 8),
+    (16, 1, 128, 16, 0, [600, 500]), (12, 4, 80, 16, 100, [330] * 4), (6, 2, 96, 48, 0, [440] * 6),
+    (3, 1, 20, 16, 0, [650] * 8), (7, 1, 36, 16, 33, [700] * 3), (32, 32, 4, 16, 1, [530]), (32, 8, 112, 16, 16, [170, 360]),
+])
+def test_prompts_in_tiles(dev, nh, nkv, hd, bs, window, sizes):
+    # prompts from their beginning, then more of each from an odd position, beside a step of another
+    rng = np.random.default_rng(nh * hd)
+    kw = dict(max_positions=1500, sliding_window=window)
+    with KvCache(dev, 1, nh, nkv, hd, block_size=bs, max_seqs=len(sizes) + 1, bits=8, **kw) as kv:
+        o = Kv8Oracle(1, nh, nkv, hd, **kw)
+        seqs = [kv.open_seq() for _ in sizes]
+        other = kv.open_seq()
+        for call, add in enumerate((0, -37)):
+            spans = [(o.seq_len(s), o.seq_len(s) + n + add) for s, n in zip(seqs, sizes)]
+            assert workgroups(nh, nkv, spans) > 1024 or call
+            ids = [s for s, (a, b) in zip(seqs, spans) for _ in range(b - a)] + [other] * call
+            q, k, v = draw(rng, len(ids), nh, nkv, hd)
+            what = f"tiles {nh}/{nkv}/{hd} bs {bs} window {window}, call {call}"
+            say(what)
+            got = kv.attention(0, ids, q, k, v)
+            o.append(0, ids, k, v)
+            at = 0
+            for s, (a, b) in zip(seqs + [other] * call, spans + [(0, 1)]):
+                mine = slice(at, at + b - a)
+                want, mag = o.attend_run(0, s, a, q[mine])
+                check(got[mine], want, mag, b, hd, np.abs(v).max() + 5, what)
+                precise(got[mine], want, what)
+                at += b - a
+        same_rows(kv, o, 0, seqs + [other], "tiles")
+
+
 @pytest.mark.parametrize("bs,window", [(16, 0), (32, 0), (64, 7), (16, 16), (16, 1), (48, 100), (16, 250)])
 def test_pages_and_windows(dev, bs, window):
     nh, nkv, hd = 8, 2, 64
@@ -155,6 +194,14 @@ def test_long_spans_join_their_splits(dev):
         for step in range(4):
             run(kv, o, 0, [a, b], draw(rng, 2, nh, nkv, hd), f"long spans, step {step}")
         run(kv, o, 0, [a] * 40 + [b], draw(rng, 41, nh, nkv, hd), "long spans, prompt beside a step")
+        # 220 tokens in tiles, their keys in many splits, the own blocks by themselves
+        assert workgroups(nh, nkv, [(5034, 5254)]) > 1024
+        q, k, v = draw(rng, 221, nh, nkv, hd)
+        got = kv.attention(0, [b] + [a] * 220, q, k, v)
+        o.append(0, [b] + [a] * 220, k, v)
+        want, mag = o.attend_run(0, a, 5034, q[1:])
+        check(got[1:], want, mag, 5254, hd, 6.0, "long spans, tiles")
+        precise(got[1:], want, "long spans, tiles")
 
 
 @pytest.mark.parametrize("order", ["interleaved", "mixed", "twice"])
@@ -302,16 +349,18 @@ def test_truncate_restores_more_sequences_than_one_launch_takes(dev):
             run(kv, o, l, s, draw(rng, n, 2, nkv, hd), "after")
 
 
+@pytest.mark.parametrize("tiles", [False, True], ids=["rows", "tiles"])
 @pytest.mark.parametrize("what", ["nan_k", "inf_k", "nan_v", "nan_q", "inf_q", "huge_q", "huge_k", "zero", "tiny", "scales"])
-def test_unusual_values(dev, what):
+def test_unusual_values(dev, what, tiles):
     """Non-finite input stands for NaN in its block; uniform weights where a score is not below +inf;
     values of very different size from block to block, and none but zeros."""
-    nh, nkv, hd = 4, 2, 32
+    nh, nkv, hd = (32, 32, 8) if tiles else (4, 2, 32)
+    assert not tiles or workgroups(nh, nkv, [(22, 562)]) > 1024
     rng = np.random.default_rng(13)
-    with KvCache(dev, 1, nh, nkv, hd, max_positions=200, max_seqs=1, bits=8) as kv:
-        o = Kv8Oracle(1, nh, nkv, hd, max_positions=200)
+    with KvCache(dev, 1, nh, nkv, hd, max_positions=700, max_seqs=1, bits=8) as kv:
+        o = Kv8Oracle(1, nh, nkv, hd, max_positions=700)
         s = kv.open_seq()
-        for call, n in enumerate((20, 1, 1, 60, 1, 15, 1, 1)):
+        for call, n in enumerate((20, 1, 1, 540 if tiles else 60, 1, 15, 1, 1)):
             q, k, v = draw(rng, n, nh, nkv, hd)
             if what == "zero":
                 k[:], v[:] = 0, 0
