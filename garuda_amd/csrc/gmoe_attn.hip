@@ -1011,12 +1011,12 @@ hipError_t launch_append(const AttnArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-// grid (chunks, n_kv), 256 threads: a chunk's rows of one kv head, keys and values. Pages
+// grid (chunks * n_kv), 256 threads: a chunk's rows of one kv head, keys and values. Pages
 // hold [2][n_kv][bs][hd] f32.
 __global__ void __launch_bounds__(256) k_kv_read(Kv8Pool p, const float* pool, const Kv8Rows* rows, Kv8RowsInline inl,
                                                  float* k, float* v) {
-  const Kv8Rows r = rows ? rows[blockIdx.x] : inl.r[blockIdx.x];
-  const uint32_t h = blockIdx.y, kvd = p.n_kv * p.hd;
+  const uint32_t i = blockIdx.x / p.n_kv, h = blockIdx.x % p.n_kv, kvd = p.n_kv * p.hd;
+  const Kv8Rows r = rows ? rows[i] : inl.r[i];
   const uint32_t page = p.tables[(size_t)r.table * p.ppseq + r.block];
   const float* src = pool + (size_t)page * 2 * p.bs * kvd + ((size_t)h * p.bs + r.r0) * p.hd;
   float* dk = k + (size_t)r.i0 * kvd + h * p.hd;
@@ -1030,7 +1030,7 @@ __global__ void __launch_bounds__(256) k_kv_read(Kv8Pool p, const float* pool, c
 
 hipError_t launch_kv_read(const Kv8Pool& p, const float* pool, const Kv8Rows* rows, const Kv8RowsInline& inl,
                           uint32_t nrows, float* k, float* v, hipStream_t st) {
-  hipLaunchKernelGGL(k_kv_read, dim3(nrows, p.n_kv), dim3(256), 0, st, p, pool, rows, inl, k, v);
+  hipLaunchKernelGGL(k_kv_read, dim3(nrows * p.n_kv), dim3(256), 0, st, p, pool, rows, inl, k, v);
   return hipGetLastError();
 }
 

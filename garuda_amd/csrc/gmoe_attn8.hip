@@ -1,8 +1,8 @@
 // gmoe_attn8.hip — the paged KV cache held in 8 bits: append, attention, reading back.
 //
 // A sequence's positions are cut into blocks of 16. Of a complete block, one kv head's keys
-// (values) x are held as codes c = rint(x * 127 / m), m = max |x| over the block's 16 rows,
-// and a scale s = m / 127 rounded to f32; they stand for c * s. The block of the sequence's
+// (values) x are held as codes c = rint(x * (127 * (1 / m))), m = max |x| over the block's 16
+// rows, and a scale s = m / 127 rounded to f32; they stand for c * s. The block of the sequence's
 // last position is also held in f32 as it was given (keys rotated): a token attends to its
 // own block's rows in f32 and to every earlier block's as held in 8 bits, so that its
 // context does not depend on how the sequence was cut into calls.
@@ -1588,10 +1588,10 @@ __global__ void __launch_bounds__(256) k8_read(Kv8Pool p, const Kv8Rows* rows, K
   }
 }
 
-// grid (blocks, n_kv), 256 threads: rows r0 .. r0 + n - 1 of a held block become open rows.
+// grid (blocks * n_kv), 256 threads: rows r0 .. r0 + n - 1 of a held block become open rows.
 __global__ void __launch_bounds__(256) k8_reopen(Kv8Pool p, Kv8RowsInline inl) {
-  const Kv8Rows r = inl.r[blockIdx.x];
-  const uint32_t h = blockIdx.y, hd = p.hd;
+  const Kv8Rows r = inl.r[blockIdx.x / p.n_kv];
+  const uint32_t h = blockIdx.x % p.n_kv, hd = p.hd;
   const size_t u = kv8_block(p, kv8_page(p, r.table, r.block), r.block, h);
   const uint8_t* c = kv8_codes(p, u);
   const float sk = p.scales[2 * u], sv = p.scales[2 * u + 1];
@@ -1642,6 +1642,14 @@ hipError_t launch_rows_of(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st
 
 }  // namespace
 
+bool kv8_fits(const Kv8Args& a, bool step) {
+  const uint64_t kv = a.p.n_kv, G = a.n_heads / kv;
+  // workgroups along x, of 256 threads
+  if (step) return kv * a.items <= kMaxWgs && (uint64_t)a.n * a.n_heads <= kMaxWgs;
+  return kv * a.njob <= kMaxWgs && a.nrun * kv * kv8_group_tokens(G) * G <= kMaxWgs && kv * a.ntile <= kMaxWgs &&
+         a.nparts <= kMaxGridYz && a.ntile <= kMaxGridYz;
+}
+
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) { return launch_rows_of<true>(a, inl, st); }
 
 hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
@@ -1672,7 +1680,7 @@ hipError_t launch_kv8_read(const Kv8Pool& p, const Kv8Rows* rows, const Kv8RowsI
 }
 
 hipError_t launch_kv8_reopen(const Kv8Pool& p, const Kv8RowsInline& inl, uint32_t nrows, hipStream_t st) {
-  hipLaunchKernelGGL(k8_reopen, dim3(nrows, p.n_kv), dim3(256), 0, st, p, inl);
+  hipLaunchKernelGGL(k8_reopen, dim3(nrows * p.n_kv), dim3(256), 0, st, p, inl);
   return hipGetLastError();
 }
 

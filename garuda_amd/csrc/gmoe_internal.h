@@ -556,6 +556,10 @@ struct Kv8Args {
 struct Kv8Inline {
   AttnEntry e[kKv8Inline];
 };
+// Whether the launches of a planned step, or call, fit a grid: at most kMaxWgs workgroups of 256
+// threads along x (threads are counted in 32 bits), kMaxGridYz along y or z.
+constexpr uint32_t kMaxWgs = 0xffffffffu / 256, kMaxGridYz = 65535;
+bool kv8_fits(const Kv8Args& a, bool step);
 // Attention of one token of each of n different sequences, appended on the way.
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st);
 // Appends the call's jobs; then attention of its runs, where a.ctx is given.

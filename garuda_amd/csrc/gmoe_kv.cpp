@@ -400,6 +400,11 @@ gmoe_status plan8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n,
   if (need > kv->free_pages.size())
     return kfail(GMOE_ERR_CACHE, "the KV pool has %zu free pages, the call needs %llu", kv->free_pages.size(),
                  (unsigned long long)need);
+  for (size_t r = 0; r < P.runs.size(); r++) {  // what commit8 may not fail at
+    std::vector<uint32_t>& pages = kv->seqs[P.seq[r]].pages[layer];
+    const size_t most = ((uint64_t)P.runs[r].pos0 + P.runs[r].n + D.block_size - 1) / D.block_size;
+    if (most > pages.capacity()) pages.reserve(std::max(most, 2 * pages.capacity()));
+  }
   return GMOE_OK;
 }
 
@@ -519,6 +524,8 @@ bool apart(const Kv8Args& a) {
   return !over(a.q, qd, a.q_stride) || (a.ctx == a.q && a.q_stride == qd);
 }
 
+gmoe_status too_many(uint32_t n) { return kfail(GMOE_ERR_INFERENCE, "%u tokens are more than one launch takes", n); }
+
 // attend() for a cache in 8 bits; with `out` null the tokens are only appended.
 gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n, const float* q, const float* k,
                     const float* v, float* out, hipStream_t st, uint32_t q_stride, uint32_t kv_stride) {
@@ -540,6 +547,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     }
     a.nparts = kv8_parts(span);
     a.fused = kv8_fused(a.items, D.n_kv_heads, a.nparts, G * D.head_dim);
+    if (!kv8_fits(a, true)) return too_many(n);
     const size_t eb = n > kKv8Inline ? (n * sizeof(AttnEntry) + 255) & ~(size_t)255 : 0;
     if (gmoe_status s = grow_scratch(kv, eb + step8_bytes(kv, n, a.nparts))) return s;
     if (eb)
@@ -567,6 +575,8 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     at += (bytes + 255) & ~(size_t)255;
     return o;
   };
+  a.njob = P.njob;
+  if (!kv8_fits(a, false)) return too_many(n);
   size_t o_run = 0, o_qr = 0, o_own = 0, o_max = 0, o_part = 0, o_tpart = 0;
   if (out) {
     cut_runs(kv, P.runs, groups, tiles);
@@ -582,6 +592,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
       a.nparts = kv8_parts(span);
       a.fused = kv8_fused(a.items, D.n_kv_heads, a.nparts, kv8_group_tokens(G) * G * D.head_dim);
     }
+    if (!kv8_fits(a, false)) return too_many(n);  // its groups and tiles
     o_run = take((groups.size() + tiles.size()) * sizeof(Kv8Run));
     o_qr = take((size_t)n * D.n_heads * D.head_dim * 4);
     o_own = take((size_t)P.njob * 2 * kKv8Block * kv->kvd * 4);
@@ -604,7 +615,6 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     }
   a.hjob = jobs;
   a.hrun = reinterpret_cast<const Kv8Run*>(pin + jb);
-  a.njob = P.njob;
   if (out) {
     a.run = reinterpret_cast<Kv8Run*>(kv->scratch + o_run);
     a.qr = reinterpret_cast<float*>(kv->scratch + o_qr);
@@ -622,6 +632,7 @@ gmoe_status append(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t n
                    hipStream_t st) {
   if (kv->q8) return attend8(kv, layer, seqs, n, nullptr, k, v, nullptr, st, 0, 0);
   if (gmoe_status s = refuse_capture(st)) return s;
+  if (n > kMaxWgs) return too_many(n);
   std::vector<AttnEntry> ent(n ? n : 1);
   uint32_t maxspan;
   if (gmoe_status s = plan(kv, layer, seqs, n, ent.data(), &maxspan)) return s;
@@ -664,6 +675,7 @@ gmoe_status read_rows(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, const u
     rows.push_back(Kv8Rows{s * D.n_layers + layer, b, i, r, 1, kv->q8 && (uint64_t)(b + 1) * kKv8Block <= len});
     more = std::min(std::min(per - r, kKv8Block), len - pos[i]) - 1;
   }
+  if (rows.size() * D.n_kv_heads > kMaxWgs) return too_many(n);
   Kv8RowsInline inl{};
   uint8_t* pin = nullptr;
   const size_t bytes = rows.size() * sizeof(Kv8Rows);
@@ -1020,6 +1032,11 @@ static gmoe_status kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, bool q8, g
   if (q8 && D.block_size % kKv8Block)
     return kfail(GMOE_ERR_MODEL, "block_size %u must be a multiple of %u, the positions that share a scale", D.block_size,
                  kKv8Block);
+  // pages have numbers of 32 bits, and 2^48 bytes are more than any card's
+  if (D.max_pages > 0xffffffffull || (double)D.max_pages * D.block_size * D.n_kv_heads * D.head_dim > 0x1p48 ||
+      (double)D.max_seqs * D.n_layers * std::max((double)D.max_positions / D.block_size, (double)D.n_kv_heads * D.head_dim) > 0x1p48)
+    return kfail(GMOE_ERR_CONFIG, "a KV cache of %llu pages and %u sequences is too large",
+                 (unsigned long long)D.max_pages, D.max_seqs);
   std::unique_ptr<gmoe_kv> kv(new gmoe_kv);
   kv->ctx = ctx;
   kv->d = D;
@@ -1058,11 +1075,11 @@ static gmoe_status kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, bool q8, g
 }
 
 gmoe_status gmoe_kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out) {
-  return kv_create(ctx, desc, false, out);
+  return guarded([&] { return kv_create(ctx, desc, false, out); });
 }
 
 gmoe_status gmoe_kv_create_q8(gmoe_ctx* ctx, const gmoe_kv_desc* desc, gmoe_kv** out) {
-  return kv_create(ctx, desc, true, out);
+  return guarded([&] { return kv_create(ctx, desc, true, out); });
 }
 
 void gmoe_kv_destroy(gmoe_kv* kv) {

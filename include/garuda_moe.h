@@ -423,7 +423,8 @@ gmoe_status gmoe_attention_async(gmoe_kv* kv, uint32_t layer, const uint32_t* se
  *
  * Of one sequence, layer and kv head, a block of 16 positions' keys (values) x is held as
  * integers rint(x * (127 * (1 / m))), m the largest |x| of the block (in 64 bits), and one f32
- * scale m / 127, and stands for their product; it is held so from the call on that appends its last position.
+ * scale m / 127, and stands for their product; it is held so from the call on that appends its
+ * last position.
  * The block that a sequence's last position is in is held in f32 besides. A token attends to
  * the positions of its own block as they were given (keys rotated), and to earlier blocks as
  * held in 8 bits, so its context does not depend on how the sequence was cut into calls
@@ -431,11 +432,11 @@ gmoe_status gmoe_attention_async(gmoe_kv* kv, uint32_t layer, const uint32_t* se
  * rotated pair rounded once to f32; gmoe_kv_create's caches form both in f32, as the
  * reference does.
  *
- * Products and weights keep f32's precision: a query, and a position's softmax weight, is
- * held as the sum of two fp16 values, to about 2^-22 of the head's largest query element
- * and of the weight (weights times the value scale that are below 2^-24 of the largest
- * lose bits, to 2^-39 of it). A block with a NaN or an infinity stands for NaN throughout;
- * scores that are NaN or +inf, or none above -inf, give uniform weights as in f32.
+ * Products run on fp16 matrix instructions, with f32 sums. A code is exact in fp16; a query
+ * element, and a position's softmax weight (times its value's scale), is the sum of two fp16
+ * values, within 2^-21 of it or 2^-32 of the largest of its head (row), whichever is more. A
+ * block with a NaN or an infinity stands for NaN throughout; scores that are NaN or +inf, or
+ * none above -inf, give uniform weights as in f32.
  *
  * block_size must be a multiple of 16. Calls that take a stream plan positions and pages on
  * the host as they are made, so they are refused while the stream is being captured. */

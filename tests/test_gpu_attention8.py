@@ -425,6 +425,29 @@ def test_refusals_change_nothing(dev):
             assert kv.free_pages() == 2
 
 
+@pytest.mark.parametrize("bits_", [8, 32])
+@pytest.mark.parametrize("more", [dict(max_pages=2**60), dict(max_pages=2**33), dict(block_size=2**31, max_pages=2**31),
+                                  dict(max_positions=2**32 - 1, max_seqs=2**31, max_pages=1)])
+def test_sizes_that_no_card_has(dev, bits_, more):
+    # their products pass 64 bits, or a page's number 32
+    with pytest.raises(G.ConfigError):
+        KvCache(dev, 1, 4, 2, 16, bits=bits_, **more)
+
+
+def test_a_call_that_no_grid_holds(dev):
+    # one head of 4, 256 rows a tile: one tile more than a grid's 65535; refused before a position is taken
+    n = 65535 * 256 + 1
+    with KvCache(dev, 1, 1, 1, 4, block_size=1 << 16, max_positions=n, max_seqs=1, bits=8) as kv, Gpu() as gpu:
+        s, free = kv.open_seq(), kv.free_pages()
+        x = gpu.up(np.zeros(4 * n, np.float32))
+        with pytest.raises(G.InferenceError, match="one launch"):
+            kv.attention_async(0, np.full(n, s, np.uint32), x, x, x, gpu.up(np.zeros(4 * n, np.float32)), gpu.stream)
+        assert kv.seq_len(s) == 0 and kv.free_pages() == free
+        kv.append_async(0, np.full(1000, s, np.uint32), x, x, gpu.stream)
+        gpu.wait()
+        assert kv.seq_len(s) == 1000
+
+
 def test_capture_is_refused(dev):
     with KvCache(dev, 1, 4, 2, 32, max_positions=64, max_seqs=1, bits=8) as kv, Gpu() as gpu:
         s = kv.open_seq()
