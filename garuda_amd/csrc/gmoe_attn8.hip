@@ -538,48 +538,52 @@ __device__ __forceinline__ float4 uniform_row(const Kv8Args& a, const Kv8Run& ru
   return make_float4(u[0], u[1], u[2], u[3]);
 }
 
-// grid (groups * n_kv * R), 256 threads: the context of one row of a group, joined from its
-// parts. kKv8Join parts at a time, in order, then what these give: in a call without this launch
-// (kv8_fused) there are no more than those.
+// 256 threads: contexts of a.jrows rows, joined from their parts: kKv8Join parts at a time,
+// in order, by hd / 4 threads, then what these give. In a call without this launch (kv8_fused) there
+// are no more than the first of those.
 template <bool STEP>
 __global__ void __launch_bounds__(256) k8_join(Kv8Args a, Kv8Inline inl) {
   __shared__ float4 go[256];
   __shared__ float gm[256], gl[256];
-  __shared__ uint32_t bad;
+  __shared__ uint32_t bad[256];
   const Kv8Pool& p = a.p;
   const Kv8Part part = rows_parts(a, STEP);
-  const uint32_t r = blockIdx.x % part.R, h = blockIdx.x / part.R % p.n_kv, x = blockIdx.x / part.R / p.n_kv;
-  Kv8Run run;
-  if (STEP) {
-    const AttnEntry e = a.ent ? a.ent[x] : inl.e[x];
-    run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
-  } else {
-    run = a.run[x];
+  const uint32_t t = threadIdx.x, hd = p.hd, q4 = hd / 4, c = t % q4, g = t / q4;
+  const uint32_t nr = a.jrows, per = 256 / q4 / nr;  // rows, and threads' groups a row
+  const uint32_t w = g / per, i = blockIdx.x * nr + w, r = i % part.R, h = i / part.R % p.n_kv, x = i / part.R / p.n_kv;
+  Kv8Run run{};
+  if (w < nr && x < part.nx) {
+    if (STEP) {
+      const AttnEntry e = a.ent ? a.ent[x] : inl.e[x];
+      run = Kv8Run{x, 1, e.pos, 0, (uint32_t)((e.pages - p.tables) / p.ppseq)};
+    } else {
+      run = a.run[x];
+    }
   }
-  const uint32_t t = threadIdx.x, hd = p.hd, q4 = hd / 4, ng = 256 / q4, g = t / q4, c = t % q4;
-  const uint32_t n = kv8_parts_of(run.pos0, kv8_start(a, run.pos0));
-  if (r >= run.n * (a.n_heads / p.n_kv)) return;
-  if (t == 0) bad = 0;
+  const bool in = r < run.n * (a.n_heads / p.n_kv);
+  const uint32_t n = in ? kv8_parts_of(run.pos0, kv8_start(a, run.pos0)) : 0;
+  bad[t] = 0;
   __syncthreads();
   Joined all;
-  for (uint32_t s0 = 0; s0 < n; s0 += ng * kKv8Join) {
+  for (uint32_t s0 = 0; s0 < a.nparts; s0 += per * kKv8Join) {
     Joined j;
-    if (g < ng) j.parts<false, 8>(part, s0 + g * kKv8Join, min(n, s0 + (g + 1) * kKv8Join), part.row(0, x, h, r), hd, c);
-    if (!j.ok) bad = 1;
+    const uint32_t s = s0 + g % per * kKv8Join;
+    j.parts<false, 8>(part, s, min(n, s + kKv8Join), part.row(0, x, h, r), hd, c);
+    if (!j.ok) bad[w] = 1;
     go[t] = j.o;
     gm[t] = j.m;
     gl[t] = j.l;
     __syncthreads();
-    if (t < q4)
-      for (uint32_t k = 0; k < ng; k++) {
-        all.raise(gm[k * q4 + t]);
-        all.add(gm[k * q4 + t], gl[k * q4 + t], go[k * q4 + t]);
+    if (in && g % per == 0)
+      for (uint32_t k = t; k < t + per * q4; k += q4) {
+        all.raise(gm[k]);
+        all.add(gm[k], gl[k], go[k]);
       }
     __syncthreads();
   }
-  if (t >= q4) return;
+  if (!in || g % per) return;
   float4 o;
-  if (!all.mean(o) || bad) o = uniform_row<STEP, false>(a, run, h, r, c);
+  if (!all.mean(o) || bad[w]) o = uniform_row<STEP, false>(a, run, h, r, c);
   put_ctx(ctx_row(a, run, h, r) + 4 * c, o);
 }
 
@@ -1618,7 +1622,11 @@ void launch_rows(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) {
   const dim3 grid(a.p.n_kv * (STEP && !one ? a.items : nx), 1, STEP || one ? 1 : a.nparts);
   auto kernel = one ? k8_rows<NS, STEP, true> : k8_rows<NS, STEP, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(256), lds, st, a, inl);
-  if (!one && !a.fused) hipLaunchKernelGGL(k8_join<STEP>, dim3(a.p.n_kv * nx * rows), dim3(256), 0, st, a, inl);
+  if (one || a.fused) return;
+  const uint32_t n = a.p.n_kv * nx * rows;
+  Kv8Args j = a;
+  j.jrows = kv8_join_rows(a.p.hd, a.nparts, n);
+  hipLaunchKernelGGL(k8_join<STEP>, dim3((n + j.jrows - 1) / j.jrows), dim3(256), 0, st, j, inl);
 }
 
 // f of the build for the heads' width

@@ -521,6 +521,13 @@ constexpr uint32_t kKv8Join = 16, kKv8FusedWgs = 1024;
 constexpr uint32_t kv8_fused(uint32_t items, uint32_t n_kv, uint32_t nparts, uint32_t floats) {  // of a group's context
   return nparts <= kKv8Join && floats <= 4 * 256 && (uint64_t)items * n_kv <= kKv8FusedWgs ? 1 : 0;
 }
+// Rows that a workgroup of the joining launch takes: hd / 4 threads for kKv8Join parts of one, so
+// several where parts are few and workgroups enough (6 sequences' 5 drafts at 3000, a row each
+// 38.2 us, several 34.6; 32 heads of 256 at 6000, 256 rows, 27.0 and 27.7).
+constexpr uint32_t kv8_join_rows(uint32_t hd, uint32_t nparts, uint64_t rows) {
+  const uint32_t groups = 256 / (hd / 4), per = (nparts + kKv8Join - 1) / kKv8Join, most = per < groups ? groups / per : 1;
+  return rows / 256 < most ? (rows < 512 ? 1 : (uint32_t)(rows / 256)) : most;
+}
 constexpr uint32_t kv8_parts_of(uint32_t pos, uint32_t start) {  // of an entry
   return 1 + (pos / kKv8Block * kKv8Block - start / kKv8Block * kKv8Block + kKv8Split - 1) / kKv8Split;
 }
@@ -550,6 +557,7 @@ struct Kv8Args {
   uint32_t* done;      // [groups][n_kv] parts that are written; 0 between calls
   uint32_t fused;      // 1: the last workgroup of a group joins its parts (kv8_fused)
   uint32_t items;      // the groups' parts, over all entries
+  uint32_t jrows;      // rows a workgroup that joins them (kv8_join_rows; set with the launch)
   float* tpart;        // of the tiles' rows: tsplits splits of tkeys positions, the first of them
   uint32_t tsplits, tkeys, town;  // the rows' own blocks alone where town is 1
 };
