@@ -231,16 +231,23 @@ __device__ __forceinline__ void hold_block(const Kv8Pool& p, size_t unit, const 
 // turned rows go to a.qr. The job of a sequence's first block writes the open rows of its last
 // one, after it has read those that were there. Copies the call's groups and tiles to the
 // device for the launches after it.
-template <int NS>
-__global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
+// I: Kv8CallInline, or without one OfHost (3 kB of arguments cost the host 0.5 us).
+struct OfHost {};
+template <int NS, class I>
+__global__ void __launch_bounds__(256) k8_append(Kv8Args a, I inl) {
+  constexpr bool INL = std::is_same<I, Kv8CallInline>::value;
   constexpr uint32_t HS = kv8_pad(32 * NS), Q4 = 8 * NS;
   __shared__ __attribute__((aligned(16))) float kt[kKv8Block * HS], vt[kKv8Block * HS];
   __shared__ uint32_t red[8];
   __shared__ Kv8Job job;
   const Kv8Pool& p = a.p;
   const uint32_t h = blockIdx.x % p.n_kv, jb = blockIdx.x / p.n_kv, t = threadIdx.x;
-  auto take = [&](uint32_t i) {  // job i, from pinned memory
-    if (t < sizeof(Kv8Job) / 4) reinterpret_cast<uint32_t*>(&job)[t] = reinterpret_cast<const uint32_t*>(a.hjob + i)[t];
+  auto take = [&](uint32_t i) {  // job i
+    auto word = [&](const Kv8Job* j) { return reinterpret_cast<const uint32_t*>(j + i)[t]; };
+    if (t < sizeof(Kv8Job) / 4) {
+      if constexpr (INL) reinterpret_cast<uint32_t*>(&job)[t] = word(inl.j);
+      else reinterpret_cast<uint32_t*>(&job)[t] = word(a.hjob);
+    }
     __syncthreads();
   };
   take(jb);
@@ -273,7 +280,10 @@ __global__ void __launch_bounds__(256) k8_append(Kv8Args a) {
   if (h == 0 && t == 0 && (flags & kKv8Fresh))
     p.tables[(size_t)job.table * p.ppseq + job.block / (p.bs / kKv8Block)] = job.page;
   if (h == 0 && a.qr)
-    for (uint32_t x = jb * 256 + t; x < a.nrun + a.ntile; x += a.njob * 256) a.run[x] = a.hrun[x];
+    for (uint32_t x = jb * 256 + t; x < a.nrun + a.ntile; x += a.njob * 256) {
+      if constexpr (INL) a.run[x] = inl.r[x];
+      else a.run[x] = a.hrun[x];
+    }
   BlockRows<NS> rows;
   auto get = [&] {
     rows.load(a, job.table, job.r0, job.n, h, [&](uint32_t r) { return job.ent[r]; });
@@ -1660,9 +1670,12 @@ bool kv8_fits(const Kv8Args& a, bool step) {
 
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st) { return launch_rows_of<true>(a, inl, st); }
 
-hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st) {
+hipError_t launch_kv8_call(const Kv8Args& a, const Kv8CallInline& inl, hipStream_t st) {
   const dim3 jobs(a.njob * a.p.n_kv, 1, a.qr ? 1 + (a.n_heads / a.p.n_kv + 3) / 4 : 1);
-  by_width(a.p.hdp, [&](auto ns) { hipLaunchKernelGGL(k8_append<ns()>, jobs, dim3(256), 0, st, a); });
+  by_width(a.p.hdp, [&](auto ns) {
+    if (a.hjob) k8_append<ns(), OfHost><<<jobs, dim3(256), 0, st>>>(a, OfHost{});
+    else k8_append<ns(), Kv8CallInline><<<jobs, dim3(256), 0, st>>>(a, inl);
+  });
   if (!a.ctx) return hipGetLastError();
   if (a.ntile) {
     const dim3 grid(a.p.n_kv, a.ntile, a.tsplits);

@@ -545,8 +545,8 @@ struct Kv8Args {
   uint32_t nsl;                  // > 1: q, k and v are sums of nsl slices sl_stride floats apart
   uint64_t sl_stride;
   float* ctx;
-  const Kv8Job* hjob;  // [njob] in pinned host memory, and the runs; k8_append copies them to
-  const Kv8Run* hrun;  //   run for the launches after it: nrun groups, then ntile tiles
+  const Kv8Job* hjob;  // [njob] in pinned host memory (null: in Kv8CallInline), and the runs; k8_append
+  const Kv8Run* hrun;  //   copies these to run for the launches after it: nrun groups, then ntile tiles
   Kv8Run* run;
   uint32_t njob, nrun, ntile;
   float* qr;           // [n][n_heads * hd] rotated queries; null: the call only appends
@@ -564,6 +564,13 @@ struct Kv8Args {
 struct Kv8Inline {
   AttnEntry e[kKv8Inline];
 };
+// A short call's jobs and runs, carried in k8_append's arguments where hjob is null: from pinned memory
+// its workgroups have them 2 us later.
+constexpr uint32_t kKv8InlineJobs = 24, kKv8InlineRuns = 32;
+struct Kv8CallInline {
+  Kv8Job j[kKv8InlineJobs];
+  Kv8Run r[kKv8InlineRuns];
+};
 // Whether the launches of a planned step, or call, fit a grid: at most kMaxWgs workgroups of 256
 // threads along x (threads are counted in 32 bits), kMaxGridYz along y or z.
 constexpr uint32_t kMaxWgs = 0xffffffffu / 256, kMaxGridYz = 65535;
@@ -571,7 +578,7 @@ bool kv8_fits(const Kv8Args& a, bool step);
 // Attention of one token of each of n different sequences, appended on the way.
 hipError_t launch_kv8_step(const Kv8Args& a, const Kv8Inline& inl, hipStream_t st);
 // Appends the call's jobs; then attention of its runs, where a.ctx is given.
-hipError_t launch_kv8_call(const Kv8Args& a, hipStream_t st);
+hipError_t launch_kv8_call(const Kv8Args& a, const Kv8CallInline& inl, hipStream_t st);
 // Rows of blocks to k and v [n][n_kv * hd]: nrows of them, in `inl` when they are at most kKv8Inline,
 // else in `rows` (memory that the device reads).
 struct Kv8RowsInline {

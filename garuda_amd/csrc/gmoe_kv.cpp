@@ -602,19 +602,22 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     if (gmoe_status s = grow_scratch(kv, at)) return s;
   }
   const size_t jb = P.njob * sizeof(Kv8Job), rb = (groups.size() + tiles.size()) * sizeof(Kv8Run);
-  if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
+  Kv8CallInline inl;
+  Kv8Job* jobs = inl.j;
+  Kv8Run* runs = inl.r;
+  if (P.njob > kKv8InlineJobs || groups.size() + tiles.size() > kKv8InlineRuns) {
+    if (gmoe_status s = take_pinned(kv, jb + rb, st, &pin)) return s;
+    a.hjob = jobs = reinterpret_cast<Kv8Job*>(pin);
+    a.hrun = runs = reinterpret_cast<Kv8Run*>(pin + jb);
+  }
   commit8(kv, layer, P);
-  Kv8Job* jobs = reinterpret_cast<Kv8Job*>(pin);
   fill_jobs(kv, layer, P, jobs);
-  Kv8Run* runs = reinterpret_cast<Kv8Run*>(pin + jb);
   for (const std::vector<Kv8Run>* v : {&groups, &tiles})
     for (Kv8Run r : *v) {  // a piece of run r.job
       const Kv8Run& of = P.runs[r.job];
       r.job = of.job + r.pos0 / kKv8Block - of.pos0 / kKv8Block;
       *runs++ = r;
     }
-  a.hjob = jobs;
-  a.hrun = reinterpret_cast<const Kv8Run*>(pin + jb);
   if (out) {
     a.run = reinterpret_cast<Kv8Run*>(kv->scratch + o_run);
     a.qr = reinterpret_cast<float*>(kv->scratch + o_qr);
@@ -623,7 +626,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     a.part = reinterpret_cast<float*>(kv->scratch + o_part);
     a.tpart = reinterpret_cast<float*>(kv->scratch + o_tpart);
   }
-  KV_TRY(launch_kv8_call(a, st));
+  KV_TRY(launch_kv8_call(a, inl, st));
   return GMOE_OK;
 }
 
