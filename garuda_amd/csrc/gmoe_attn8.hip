@@ -1136,16 +1136,19 @@ __device__ __forceinline__ float max32(float v) {
   return fmaxf(p.a, p.b);
 }
 __device__ __forceinline__ Kv8Part tile_parts(const Kv8Args& a) {
-  return parts_of(a, a.tpart, a.tsplits, a.ntile, kKv8TileRows);
+  return parts_of(a, a.tpart, a.tsplits, a.ntile, kv8_tile_rows(a.p.hd));
 }
 
 template <int NS>
-__global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
+__global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(Kv8Args a) {
+  constexpr uint32_t W = kv8_tile_rows(32 * NS) / 32, NT = 64 * W;             // waves and threads
   constexpr uint32_t HDP = 32 * NS, KS = HDP / 16, NP = NS / 2, CH = HDP / 8;  // CH: 16-byte columns of a key row
   constexpr uint32_t KX = CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;             // keys' column x is at x ^ (key % KX)
   constexpr uint32_t KB = 64 * HDP * 2, BUF = 2 * KB;                          // bytes of a tile's keys; of a buffer
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
-  __shared__ u32x4 qlo[8 * KS * 64];  // the queries' second halves: in registers they would spill
+  // the queries' second halves: with two waves a SIMD they would spill
+  constexpr bool QL = NS <= 4;
+  __shared__ u32x4 qlo[QL ? W * KS * 64 : 1];
   __shared__ float2 sc[2][4];
   __shared__ uint32_t marks[8];  // rows to be summed again, a bit each
   const Kv8Pool& p = a.p;
@@ -1165,60 +1168,77 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   const uint32_t row = 32 * wave + l32, rr = min(row, rows - 1), pos = pos0 + rr / G;
   const uint32_t start = start_of(pos), own = own_of(pos);
   const Kv8Part part = tile_parts(a);
-  const size_t prow = part.row(z, x, h, row);  // 256 rows a kv head
+  const size_t prow = part.row(z, x, h, row);
   const bool mine = row < rows, busy = 32 * wave < rows;
   if (!owns && lo >= hi) return;
   // what the wave's rows attend to of the held blocks: from its first row's start to its last row's own block
   const uint32_t pw0 = pos0 + min(32 * wave, rows - 1) / G, pw1 = pos0 + min(32 * wave + 31, rows - 1) / G;
   const uint32_t w_lo = start_of(pw0), w_hi = min(own_of(pw1), hi), w_in0 = start_of(pw1), w_in1 = min(own_of(pw0), hi);
 
-  // the thread's 16 bytes of codes of a tile: block sb, column sx of its HDP; the page looked up
-  // a tile ahead
-  const uint32_t sb = t / HDP, sx = t % HDP;
-  const bool stage = sb < 4;
+  // the thread's 16 byte pieces of codes of a tile: of block sb, column sx of its HDP; the pages
+  // looked up a tile ahead
+  constexpr uint32_t NY = (4 * HDP + NT - 1) / NT;
+  auto sb = [&](uint32_t y) { return (t + NT * y) / HDP; };
+  auto sx = [&](uint32_t y) { return (t + NT * y) % HDP; };
+  auto staged = [&](uint32_t y) { return 4 * HDP % NT == 0 || sb(y) < 4; };
+  size_t unit[NY];
   auto find = [&](uint32_t kb) {
-    const uint32_t b = min(kb + kKv8Block * min(sb, 3u), hi - 1) / kKv8Block;
-    return kv8_block(p, kv8_page(p, table, b), b, h);
-  };
-  uint4 kc, vc;
-  float2 sv2;
-  auto load = [&](size_t unit) {
-    const uint8_t* c = p.codes + unit * (2 * kKv8Block * HDP) + sx * 16;
-    if (stage) {
-      kc = *reinterpret_cast<const uint4*>(c);
-      vc = *reinterpret_cast<const uint4*>(c + kKv8Block * HDP);
-      sv2 = reinterpret_cast<const float2*>(p.scales)[unit];
+#pragma unroll
+    for (uint32_t y = 0; y < NY; y++) {
+      const uint32_t b = min(kb + kKv8Block * min(sb(y), 3u), hi - 1) / kKv8Block;
+      unit[y] = kv8_block(p, kv8_page(p, table, b), b, h);
     }
   };
-  uint32_t krow, kcol;  // the keys' row in its block and first 16-byte column
-  if (NS % 2 && sx >= 64 * NP) {
-    krow = (sx - 64 * NP) / 2;
-    kcol = 8 * NP + 2 * (sx % 2);
-  } else {
-    krow = sx % 64 / 4;
-    kcol = 8 * (sx / 64) + 2 * (sx % 4);
+  uint4 kc[NY], vc[NY];
+  float2 sv2[NY];
+  auto load = [&]() {
+#pragma unroll
+    for (uint32_t y = 0; y < NY; y++) {
+      const uint8_t* c = p.codes + unit[y] * (2 * kKv8Block * HDP) + sx(y) * 16;
+      if (staged(y)) {
+        kc[y] = *reinterpret_cast<const uint4*>(c);
+        vc[y] = *reinterpret_cast<const uint4*>(c + kKv8Block * HDP);
+        sv2[y] = reinterpret_cast<const float2*>(p.scales)[unit[y]];
+      }
+    }
+  };
+  uint32_t krow[NY], kcol[NY];  // the keys' row in its block and first 16-byte column
+#pragma unroll
+  for (uint32_t y = 0; y < NY; y++) {
+    const uint32_t c = sx(y);
+    if (NS % 2 && c >= 64 * NP) {
+      krow[y] = (c - 64 * NP) / 2;
+      kcol[y] = 8 * NP + 2 * (c % 2);
+    } else {
+      krow[y] = c % 64 / 4;
+      kcol[y] = 8 * (c / 64) + 2 * (c % 4);
+    }
   }
   auto store = [&](uint32_t b) {
-    if (!stage) return;
     uint8_t* buf = lds + b * BUF;
-    const uint32_t key = kKv8Block * sb + krow;
-    *reinterpret_cast<f16x8*>(buf + key * HDP * 2 + ((kcol ^ (key % KX)) * 16)) = codes8(kc.x, kc.y);
-    *reinterpret_cast<f16x8*>(buf + key * HDP * 2 + (((kcol + 1) ^ (key % KX)) * 16)) = codes8(kc.z, kc.w);
-    *reinterpret_cast<f16x8*>(buf + KB + sx * 128 + (((2 * sb) ^ (sx % 8)) * 16)) = codes8(vc.x, vc.y);
-    *reinterpret_cast<f16x8*>(buf + KB + sx * 128 + (((2 * sb + 1) ^ (sx % 8)) * 16)) = codes8(vc.z, vc.w);
-    if (sx == 0) sc[b][sb] = sv2;
+#pragma unroll
+    for (uint32_t y = 0; y < NY; y++) {
+      if (!staged(y)) continue;
+      const uint32_t s4 = sb(y), c = sx(y), key = kKv8Block * s4 + krow[y];
+      uint8_t *kd = buf + key * HDP * 2, *vd = buf + KB + c * 128;
+      *reinterpret_cast<f16x8*>(kd + ((kcol[y] ^ (key % KX)) * 16)) = codes8(kc[y].x, kc[y].y);
+      *reinterpret_cast<f16x8*>(kd + (((kcol[y] + 1) ^ (key % KX)) * 16)) = codes8(kc[y].z, kc[y].w);
+      *reinterpret_cast<f16x8*>(vd + (((2 * s4) ^ (c % 8)) * 16)) = codes8(vc[y].x, vc[y].y);
+      *reinterpret_cast<f16x8*>(vd + (((2 * s4 + 1) ^ (c % 8)) * 16)) = codes8(vc[y].z, vc[y].w);
+      if (c == 0) sc[b][s4] = sv2[y];
+    }
   };
   const bool any = !(a.town && owns) && lo < hi;
-  size_t unit = 0;
   if (any) {
-    unit = find(lo);
-    load(unit);
-    unit = find(lo + 64);
+    find(lo);
+    load();
+    find(lo + 64);
   }
   // queries: the wave's B operand
   f16x8 qh[KS];
-  u32x4* qlw = qlo + wave * KS * 64 + lane;
-  auto ql = [&](uint32_t st) { return __builtin_bit_cast(f16x8, qlw[64 * st]); };
+  f16x8 qr[QL ? 1 : KS];
+  u32x4* qlw = qlo + (QL ? wave * KS * 64 + lane : 0);
+  auto ql = [&](uint32_t st) { return QL ? __builtin_bit_cast(f16x8, qlw[64 * st]) : qr[QL ? 0 : st]; };
   float cq;
   bool odd;
   {
@@ -1250,7 +1270,8 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         for (int y = 0; y < 8; y++) f[y] = 0.0f;
       f16x8 lo8;
       split8(f, qh[s], lo8);
-      qlw[64 * s] = __builtin_bit_cast(u32x4, lo8);  // a lane's own
+      if (QL) qlw[64 * s] = __builtin_bit_cast(u32x4, lo8);  // a lane's own
+      else qr[QL ? 0 : s] = lo8;
     }
   }
   f32x16 o[NS];
@@ -1374,8 +1395,8 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
   for (uint32_t kb = lo; any && kb < hi; kb += 64, buf ^= 1) {
     const bool more = kb + 64 < hi;
     if (more) {
-      load(unit);
-      if (kb + 128 < hi) unit = find(kb + 128);
+      load();
+      if (kb + 128 < hi) find(kb + 128);
     }
     if (busy && kb < w_hi && kb + 64 > w_lo) {
       step(kb, buf);
@@ -1406,7 +1427,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         return a.own + (((size_t)job * 2 + kv) * p.n_kv + h) * kKv8Block * hd;
       };
       __syncthreads();
-      for (uint32_t it = t; it < 32 * (HDP / 4); it += 512) {
+      for (uint32_t it = t; it < 32 * (HDP / 4); it += NT) {
         const uint32_t key = it / (HDP / 4), d = it % (HDP / 4) * 4;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (d < hd && !(key < 16 ? wild[0] : wild[1])) v = *reinterpret_cast<const float4*>(src(key / 16, 0) + key % 16 * hd + d);
@@ -1419,7 +1440,7 @@ __global__ void __launch_bounds__(512, 2) k8_tile(Kv8Args a) {
         *reinterpret_cast<u32x2*>(dst) = u32x2{hi2[0], hi2[1]};
         *reinterpret_cast<u32x2*>(dst + PK) = u32x2{lo2[0], lo2[1]};
       }
-      for (uint32_t it = t; it < 16 * (HDP / 4); it += 512) {
+      for (uint32_t it = t; it < 16 * (HDP / 4); it += NT) {
         const uint32_t kp = it % 16, d = it / 16 * 4, key = 2 * kp;
         float4 v0 = make_float4(0.0f, 0.0f, 0.0f, 0.0f), v1 = v0;
         if (d < hd && !(key < 16 ? wild[0] : wild[1])) {  // 0 times a NaN would reach the other block's rows
@@ -1680,14 +1701,11 @@ hipError_t launch_kv8_call(const Kv8Args& a, const Kv8CallInline& inl, hipStream
   if (a.ntile) {
     const dim3 grid(a.p.n_kv, a.ntile, a.tsplits);
     const uint32_t rpw = 256 / (a.p.hd / 4);
-    switch (a.p.hdp / 32) {
-      case 1: hipLaunchKernelGGL(k8_tile<1>, grid, dim3(512), 0, st, a); break;
-      case 2: hipLaunchKernelGGL(k8_tile<2>, grid, dim3(512), 0, st, a); break;
-      case 3: hipLaunchKernelGGL(k8_tile<3>, grid, dim3(512), 0, st, a); break;
-      default: hipLaunchKernelGGL(k8_tile<4>, grid, dim3(512), 0, st, a); break;
-    }
+    by_width(a.p.hdp, [&](auto ns) {
+      hipLaunchKernelGGL(k8_tile<ns()>, grid, dim3(2 * kv8_tile_rows(32 * ns())), 0, st, a);
+    });
     if (a.tsplits > 1)
-      hipLaunchKernelGGL(k8_join_tile, dim3(a.ntile * a.p.n_kv, (kKv8TileRows + rpw - 1) / rpw), dim3(256), 0, st, a);
+      hipLaunchKernelGGL(k8_join_tile, dim3(a.ntile * a.p.n_kv, (kv8_tile_rows(a.p.hd) + rpw - 1) / rpw), dim3(256), 0, st, a);
   }
   return a.nrun ? launch_rows_of<false>(a, Kv8Inline{}, st) : hipGetLastError();
 }

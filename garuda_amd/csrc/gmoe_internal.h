@@ -499,7 +499,7 @@ struct Kv8Job {
   uint32_t ent[kKv8Block];
 };
 // Consecutive entries of one sequence, from entry i0 and position pos0 on; job: of pos0's block.
-// A group: at most kv8_group_tokens of one block. A tile: at most kv8_tile_tokens.
+// A group: at most kv8_group_tokens of one block. A tile: at most kv8_tile_rows of (token, query head).
 struct Kv8Run {
   uint32_t i0, n, pos0, job, table;
 };
@@ -532,8 +532,7 @@ constexpr uint32_t kv8_parts_of(uint32_t pos, uint32_t start) {  // of an entry
   return 1 + (pos / kKv8Block * kKv8Block - start / kKv8Block * kKv8Block + kKv8Split - 1) / kKv8Split;
 }
 constexpr uint32_t kv8_group_tokens(uint32_t heads) { return 16 / heads; }  // of 16 rows
-constexpr uint32_t kKv8TileRows = 256, kKv8TileHd = 128;  // and the widest heads that tiles take
-constexpr uint32_t kv8_tile_tokens(uint32_t heads) { return kKv8TileRows / heads; }
+constexpr uint32_t kv8_tile_rows(uint32_t hd) { return hd <= 128 ? 256 : 128; }  // a wave's rows are 32
 constexpr uint32_t kKv8Inline = 64;  // entries, or blocks of a read, carried in the kernel arguments
 struct Kv8Args {
   Kv8Pool p;

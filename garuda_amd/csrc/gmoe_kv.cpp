@@ -464,7 +464,7 @@ void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
 constexpr uint32_t kKv8TileMin = 48, kKv8GroupWgs = 1024;
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
   const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads, T = kv8_group_tokens(G), w = kv->d.sliding_window;
-  auto large = [&](const Kv8Run& r) { return kv->d.head_dim <= kKv8TileHd && (uint64_t)r.n * G >= kKv8TileMin; };
+  auto large = [&](const Kv8Run& r) { return (uint64_t)r.n * G >= kKv8TileMin; };
   uint64_t wgs = 0;
   for (const Kv8Run& r : runs)
     if (large(r)) {
@@ -476,7 +476,7 @@ void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv
     const bool tile = wgs > kKv8GroupWgs && large(r);
     for (uint32_t at = 0, m; at < r.n; at += m) {
       const uint32_t pos = r.pos0 + at;
-      m = std::min(r.n - at, tile ? kv8_tile_tokens(G) : std::min(T, kKv8Block - pos % kKv8Block));
+      m = std::min(r.n - at, tile ? kv8_tile_rows(kv->d.head_dim) / G : std::min(T, kKv8Block - pos % kKv8Block));
       (tile ? tiles : groups).push_back(Kv8Run{r.i0 + at, m, pos, i, r.table});
     }
   }
@@ -598,7 +598,7 @@ gmoe_status attend8(gmoe_kv* kv, uint32_t layer, const uint32_t* seqs, uint32_t 
     o_own = take((size_t)P.njob * 2 * kKv8Block * kv->kvd * 4);
     o_max = take((size_t)P.njob * D.n_kv_heads * sizeof(float2));
     o_part = take(part8_bytes(kv, groups.size(), kv8_group_tokens(G) * G, a.nparts));
-    o_tpart = take(part8_bytes(kv, tiles.size(), kKv8TileRows, a.tsplits));
+    o_tpart = take(part8_bytes(kv, tiles.size(), kv8_tile_rows(D.head_dim), a.tsplits));
     if (gmoe_status s = grow_scratch(kv, at)) return s;
   }
   const size_t jb = P.njob * sizeof(Kv8Job), rb = (groups.size() + tiles.size()) * sizeof(Kv8Run);

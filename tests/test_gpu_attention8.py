@@ -126,17 +126,20 @@ def test_steps_and_prompts_of_every_head_layout(dev, nh, nkv, hd):
         assert kv.seq_len(seqs[0], 0) == 0
 
 
-def workgroups(nh, nkv, spans):
+def workgroups(nh, nkv, spans, window=0):
     """Groups of 16 rows and splits of their spans that a call of runs (start, end) would make: above 1024 of
     them, runs of 48 rows and more go in tiles."""
     g = nh // nkv
-    return sum(-(-(e - s) // (16 // g)) * (1 + -(-((e - 1) // BLOCK * BLOCK) // 512)) * nkv for s, e in spans)
+    first = [max(0, e - window) // BLOCK * BLOCK if window else 0 for _, e in spans]
+    return sum(-(-(e - s) // (16 // g)) * (1 + -(-((e - 1) // BLOCK * BLOCK - f) // 512)) * nkv for (s, e), f in zip(spans, first))
 
 
 @pytest.mark.parametrize("nh,nkv,hd,bs,window,sizes", [
     (8, 2, 64, 16, 0, [300] * 8), (32, 8, 128, 16, 0, [150, 400]), (4, 4, 32, 32, 0, [520] * 8),
     (16, 1, 128, 16, 0, [600, 500]), (12, 4, 80, 16, 100, [330] * 4), (6, 2, 96, 48, 0, [440] * 6),
     (3, 1, 20, 16, 0, [650] * 8), (7, 1, 36, 16, 33, [700] * 3), (32, 32, 4, 16, 1, [530]), (32, 8, 112, 16, 16, [170, 360]),
+    (8, 1, 256, 16, 0, [500, 500, 300]), (4, 2, 160, 32, 50, [440] * 6), (16, 16, 192, 16, 0, [530]),
+    (5, 1, 252, 16, 0, [650] * 3), (12, 3, 132, 16, 1, [300] * 6),
 ])
 def test_prompts_in_tiles(dev, nh, nkv, hd, bs, window, sizes):
     # prompts from their beginning, then more of each from an odd position, beside a step of another
@@ -148,7 +151,7 @@ def test_prompts_in_tiles(dev, nh, nkv, hd, bs, window, sizes):
         other = kv.open_seq()
         for call, add in enumerate((0, -37)):
             spans = [(o.seq_len(s), o.seq_len(s) + n + add) for s, n in zip(seqs, sizes)]
-            assert workgroups(nh, nkv, spans) > 1024 or call
+            assert workgroups(nh, nkv, spans, window) > 1024 or call
             ids = [s for s, (a, b) in zip(seqs, spans) for _ in range(b - a)] + [other] * call
             q, k, v = draw(rng, len(ids), nh, nkv, hd)
             what = f"tiles {nh}/{nkv}/{hd} bs {bs} window {window}, call {call}"
@@ -349,12 +352,12 @@ def test_truncate_restores_more_sequences_than_one_launch_takes(dev):
             run(kv, o, l, s, draw(rng, n, 2, nkv, hd), "after")
 
 
-@pytest.mark.parametrize("tiles", [False, True], ids=["rows", "tiles"])
+@pytest.mark.parametrize("tiles", [0, 8, 132], ids=["rows", "tiles", "tiles-wide"])
 @pytest.mark.parametrize("what", ["nan_k", "inf_k", "nan_v", "nan_q", "inf_q", "huge_q", "huge_k", "zero", "tiny", "scales"])
 def test_unusual_values(dev, what, tiles):
     """Non-finite input stands for NaN in its block; uniform weights where a score is not below +inf;
     values of very different size from block to block, and none but zeros."""
-    nh, nkv, hd = (32, 32, 8) if tiles else (4, 2, 32)
+    nh, nkv, hd = (32, 32, tiles) if tiles else (4, 2, 32)
     assert not tiles or workgroups(nh, nkv, [(22, 562)]) > 1024
     rng = np.random.default_rng(13)
     with KvCache(dev, 1, nh, nkv, hd, max_positions=700, max_seqs=1, bits=8) as kv:
