@@ -1107,12 +1107,13 @@ __device__ __forceinline__ void rows_again(const Kv8Args& a, const Kv8Run& run, 
 }
 
 // ---------------------------------------------------------------------------------
-// Attention of a prompt: tiles of up to 256 (token, query head) rows of one kv head.
+// Attention of a prompt: tiles of up to 256 (token, query head) rows of one kv head, of heads wider
+// than 128 up to 128.
 //
-// One workgroup a (kv head, tile, split of the keys), 8 waves of 32 rows. The groups above
-// read a kv head's codes once for 16 rows; here 64 positions at a time go through LDS for
-// 256, converted to fp16 once (16 KB of keys and 16 of values transposed, two buffers: the
-// next tile's codes are in registers while this one's products run). Products as above, on
+// One workgroup a (kv head, tile, split of the keys), 8 waves (4) of 32 rows. The groups above
+// read a kv head's codes once for 16 rows; here 64 positions (32) at a time go through LDS for
+// all rows, converted to fp16 once (16 KB of keys and 16 of values transposed, two buffers: the
+// next step's codes are in registers while this one's products run). Products as above, on
 // v_mfma_f32_32x32x16_f16: S^T = K Q^T with the rows of A in such an order that a lane's
 // 16 scores of 32 positions are 8 consecutive ones of each of two blocks, its own half of
 // the second product's B operand; O^T = V^T P^T.
@@ -1121,6 +1122,11 @@ __device__ __forceinline__ void rows_again(const Kv8Args& a, const Kv8Run& run, 
 // two for each block, as two fp16 each, three of the four products of two such sums (the
 // fourth is 2^-22 of the first). A row that meets a score that is NaN or +inf, or whose own block
 // has a value that is not finite, is marked and summed again by itself in f32 (row_again).
+//
+// The sums of 32 rows of 256 are half the registers that a SIMD has for one wave: it runs alone, its
+// accumulation registers hold them and the queries' first halves, and nothing but the order of its
+// instructions hides the reads of LDS (1024 tokens at 8192, 8 heads of 256 on one: 309 us as the
+// compiler puts them, 254 so; in groups 559).
 //
 // Grid x is the kv head: workgroups go round-robin over the 8 XCDs, so with 8 kv heads a
 // head's codes are read into one XCD's L2.
@@ -1144,12 +1150,11 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
   constexpr uint32_t W = kv8_tile_rows(32 * NS) / 32, NT = 64 * W;             // waves and threads
   constexpr uint32_t HDP = 32 * NS, KS = HDP / 16, NP = NS / 2, CH = HDP / 8;  // CH: 16-byte columns of a key row
   constexpr uint32_t KX = CH % 16 == 0 ? 16 : CH % 8 == 0 ? 8 : 4;             // keys' column x is at x ^ (key % KX)
-  constexpr uint32_t KB = 64 * HDP * 2, BUF = 2 * KB;                          // bytes of a tile's keys; of a buffer
+  constexpr uint32_t PS = NS <= 4 ? 64 : 32, NB = PS / 16;                     // a step's positions, and blocks
+  constexpr uint32_t KB = PS * HDP * 2, VB = PS * 2, BUF = 2 * KB;             // bytes of its keys; of a dim's values; of a buffer
   __shared__ __attribute__((aligned(16))) uint8_t lds[2 * BUF];
-  // the queries' second halves: with two waves a SIMD they would spill
-  constexpr bool QL = NS <= 4;
-  __shared__ u32x4 qlo[QL ? W * KS * 64 : 1];
-  __shared__ float2 sc[2][4];
+  __shared__ u32x4 qlo[W * KS * 64];  // the queries' second halves: in registers they would spill
+  __shared__ float2 sc[2][NB];
   __shared__ uint32_t marks[8];  // rows to be summed again, a bit each
   const Kv8Pool& p = a.p;
   const uint32_t h = blockIdx.x, x = blockIdx.y, z = blockIdx.z, t = threadIdx.x, hd = p.hd, G = a.n_heads / p.n_kv;
@@ -1177,15 +1182,16 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
 
   // the thread's 16 byte pieces of codes of a tile: of block sb, column sx of its HDP; the pages
   // looked up a tile ahead
-  constexpr uint32_t NY = (4 * HDP + NT - 1) / NT;
+  constexpr uint32_t NY = (NB * HDP + NT - 1) / NT;
+  auto vcol = [](uint32_t d, uint32_t x) { return (x ^ (PS == 64 ? d % 8 : d / 2 % 4)) * 16; };
   auto sb = [&](uint32_t y) { return (t + NT * y) / HDP; };
   auto sx = [&](uint32_t y) { return (t + NT * y) % HDP; };
-  auto staged = [&](uint32_t y) { return 4 * HDP % NT == 0 || sb(y) < 4; };
+  auto staged = [&](uint32_t y) { return NB * HDP % NT == 0 || sb(y) < NB; };
   size_t unit[NY];
   auto find = [&](uint32_t kb) {
 #pragma unroll
     for (uint32_t y = 0; y < NY; y++) {
-      const uint32_t b = min(kb + kKv8Block * min(sb(y), 3u), hi - 1) / kKv8Block;
+      const uint32_t b = min(kb + kKv8Block * min(sb(y), NB - 1), hi - 1) / kKv8Block;
       unit[y] = kv8_block(p, kv8_page(p, table, b), b, h);
     }
   };
@@ -1220,11 +1226,11 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
     for (uint32_t y = 0; y < NY; y++) {
       if (!staged(y)) continue;
       const uint32_t s4 = sb(y), c = sx(y), key = kKv8Block * s4 + krow[y];
-      uint8_t *kd = buf + key * HDP * 2, *vd = buf + KB + c * 128;
+      uint8_t *kd = buf + key * HDP * 2, *vd = buf + KB + c * VB;
       *reinterpret_cast<f16x8*>(kd + ((kcol[y] ^ (key % KX)) * 16)) = codes8(kc[y].x, kc[y].y);
       *reinterpret_cast<f16x8*>(kd + (((kcol[y] + 1) ^ (key % KX)) * 16)) = codes8(kc[y].z, kc[y].w);
-      *reinterpret_cast<f16x8*>(vd + (((2 * s4) ^ (c % 8)) * 16)) = codes8(vc[y].x, vc[y].y);
-      *reinterpret_cast<f16x8*>(vd + (((2 * s4 + 1) ^ (c % 8)) * 16)) = codes8(vc[y].z, vc[y].w);
+      *reinterpret_cast<f16x8*>(vd + vcol(c, 2 * s4)) = codes8(vc[y].x, vc[y].y);
+      *reinterpret_cast<f16x8*>(vd + vcol(c, 2 * s4 + 1)) = codes8(vc[y].z, vc[y].w);
       if (c == 0) sc[b][s4] = sv2[y];
     }
   };
@@ -1232,13 +1238,12 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
   if (any) {
     find(lo);
     load();
-    find(lo + 64);
+    find(lo + PS);
   }
   // queries: the wave's B operand
   f16x8 qh[KS];
-  f16x8 qr[QL ? 1 : KS];
-  u32x4* qlw = qlo + (QL ? wave * KS * 64 + lane : 0);
-  auto ql = [&](uint32_t st) { return QL ? __builtin_bit_cast(f16x8, qlw[64 * st]) : qr[QL ? 0 : st]; };
+  u32x4* qlw = qlo + wave * KS * 64 + lane;
+  auto ql = [&](uint32_t st) { return __builtin_bit_cast(f16x8, qlw[64 * st]); };
   float cq;
   bool odd;
   {
@@ -1270,8 +1275,12 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
         for (int y = 0; y < 8; y++) f[y] = 0.0f;
       f16x8 lo8;
       split8(f, qh[s], lo8);
-      if (QL) qlw[64 * s] = __builtin_bit_cast(u32x4, lo8);  // a lane's own
-      else qr[QL ? 0 : s] = lo8;
+      qlw[64 * s] = __builtin_bit_cast(u32x4, lo8);  // a lane's own
+      if (NS > 4) {  // in accumulation registers, which the products read as well
+        u32x4 b = __builtin_bit_cast(u32x4, qh[s]);
+        asm("" : "+a"(b));
+        qh[s] = __builtin_bit_cast(f16x8, b);
+      }
     }
   }
   f32x16 o[NS];
@@ -1311,9 +1320,12 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
         ev = en;
       }
 #pragma unroll
-      for (int d = 0; d < NS; d++)
+      for (int d = 0; d < NS; d++) {
+        if (NS > 4) asm volatile("" : "+a"(o[d]));
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] *= f;
+        if (NS > 4) asm volatile("" : "+a"(o[d]));
+      }
     }
     const float mu = M == -INFINITY ? 0.0f : M, un = pow2(-ev);
     float sum = 0.0f;
@@ -1329,40 +1341,50 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
     }
     L += sum;
   };
-  // 64 held positions from kb on, in a buffer
+  // PS held positions from kb on, in a buffer
   auto step = [&](uint32_t kb, uint32_t b) {
     const uint8_t* kbuf = lds + b * BUF;
-    float s[32], w[32], svn[4], ck[4];
+    float s[PS / 2], w[PS / 2], svn[NB], ck[NB];
     int en = -100;
 #pragma unroll
-    for (uint32_t y = 0; y < 4; y++) {
+    for (uint32_t y = 0; y < NB; y++) {
       const uint32_t c = (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(sc[b][y].x));
       const uint32_t v = (uint32_t)__builtin_amdgcn_readfirstlane(__float_as_int(sc[b][y].y));
       ck[y] = above0(__uint_as_float(c) * cq);
       svn[y] = __uint_as_float(v);
       en = max(en, pow2_of(__uint_as_float(v)));
     }
-    f32x16 acc[2] = {(f32x16)(0.0f), (f32x16)(0.0f)};
+    f32x16 acc[PS / 32];
+#pragma unroll
+    for (uint32_t y = 0; y < PS / 32; y++) acc[y] = (f32x16)(0.0f);
 #pragma unroll
     for (uint32_t st = 0; st < KS; st++) {
       const f16x8 lo8 = ql(st);
 #pragma unroll
-      for (uint32_t y = 0; y < 2; y++) {
+      for (uint32_t y = 0; y < PS / 32; y++) {
         const uint32_t key = 32 * y + arow;
         const f16x8 kf = *reinterpret_cast<const f16x8*>(kbuf + key * HDP * 2 + (((2 * st + hf) ^ (key % KX)) * 16));
         acc[y] = mfma32(kf, lo8, acc[y]);
         acc[y] = mfma32(kf, qh[st], acc[y]);
       }
     }
+    if (NS > 4) {  // reads of LDS three products' operands ahead
+      __builtin_amdgcn_sched_group_barrier(0x100, 8, 0);
 #pragma unroll
-    for (uint32_t y = 0; y < 2; y++)
+      for (uint32_t st = 0; st < KS; st++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      }
+    }
+#pragma unroll
+    for (uint32_t y = 0; y < PS / 32; y++)
 #pragma unroll
       for (uint32_t r = 0; r < 16; r++) s[16 * y + r] = acc[y][r];
-    if (kb < w_in0 || kb + 64 > w_in1) {  // some row of the wave does not attend to all
+    if (kb < w_in0 || kb + PS > w_in1) {  // some row of the wave does not attend to all
       asm volatile("");                   // a branch: the selects of every tile were a fifth of its instructions
       const uint32_t top = min(own, hi);
 #pragma unroll
-      for (uint32_t y = 0; y < 4; y++) {
+      for (uint32_t y = 0; y < NB; y++) {
         const uint32_t k0 = kb + 16 * y;
         if (k0 >= top || k0 + 16 <= start) {
           svn[y] = 0.0f;
@@ -1375,30 +1397,41 @@ __global__ void __launch_bounds__(NS <= 4 ? 512 : 256, NS <= 4 ? 2 : 1) k8_tile(
         }
       }
     }
-    soften(s, 32, ck, svn, en, w);
+    soften(s, PS / 2, ck, svn, en, w);
 #pragma unroll
-    for (uint32_t y = 0; y < 4; y++) {
+    for (uint32_t y = 0; y < NB; y++) {
       f16x8 wh, wl;
       split8(w + 8 * y, wh, wl);
 #pragma unroll
       for (uint32_t d = 0; d < NS; d++) {
         const uint32_t dr = 32 * d + l32;
-        const f16x8 vf = *reinterpret_cast<const f16x8*>(kbuf + KB + dr * 128 + (((2 * y + hf) ^ (dr % 8)) * 16));
+        const f16x8 vf = *reinterpret_cast<const f16x8*>(kbuf + KB + dr * VB + vcol(dr, 2 * y + hf));
         o[d] = mfma32(vf, wl, o[d]);
         o[d] = mfma32(vf, wh, o[d]);
+      }
+    }
+    if (NS > 4) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 4, 1);
+#pragma unroll
+      for (uint32_t st = 0; st < NB * NS; st++) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 2, 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 1);
       }
     }
   };
   if (any) store(0);
   __syncthreads();
   uint32_t buf = 0;
-  for (uint32_t kb = lo; any && kb < hi; kb += 64, buf ^= 1) {
-    const bool more = kb + 64 < hi;
+  for (uint32_t kb = lo; any && kb < hi; kb += PS, buf ^= 1) {
+    const bool more = kb + PS < hi;
+    if (NS > 4)  // the sums in accumulation registers here and in soften: 256 moves a step otherwise
+#pragma unroll
+      for (int d = 0; d < NS; d++) asm("" : "+a"(o[d]));
     if (more) {
       load();
-      if (kb + 128 < hi) find(kb + 128);
+      if (kb + 2 * PS < hi) find(kb + 2 * PS);
     }
-    if (busy && kb < w_hi && kb + 64 > w_lo) {
+    if (busy && kb < w_hi && kb + PS > w_lo) {
       step(kb, buf);
     }
     if (more) store(buf ^ 1);

@@ -455,13 +455,16 @@ void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
 }
 
 // The runs cut into groups (job: the run's index, for now) of at most 16 rows, or into tiles of
-// at most 256. A group reads the cache for itself, but a call of few groups has them all on the
-// card at once, where a tile's waves without rows idle; so runs of 48 rows or more go in tiles
-// where as groups they would make more workgroups than two a CU twice over. 32 heads on 8 of
-// 128, in groups and in tiles: 32 tokens at 3008 (448 workgroups) 31 and 36 us, at 12000 (1600)
-// 53 and 49; 16 tokens of each of 6 sequences at 3008 (1344) 55.5 and 53.7, 32 of each 88 and
-// 58; 12 of each (1008) 46 and 52. 64 tokens at 2000, 8 heads on 2 of 32 (160): 19.5 and 27.
-constexpr uint32_t kKv8TileMin = 48, kKv8GroupWgs = 1024;
+// at most kv8_tile_rows. A group reads the cache for itself, but a call of few groups has them all on
+// the card at once, where a tile's waves without rows idle; so runs of 48 rows or more go in tiles
+// where as groups they would make more workgroups than the CUs hold (two each, of heads wider than 128
+// one) twice over. 32 heads on 8 of 128, in groups and in tiles: 32 tokens at 3008 (448 workgroups)
+// 31 and 36 us, at 12000 (1600) 53 and 49; 16 tokens of each of 6 sequences at 3008 (1344) 55.5 and
+// 53.7, 32 of each 88 and 58; 12 of each (1008) 46 and 52. 64 tokens at 2000, 8 heads on 2 of 32
+// (160): 19.5 and 27. 8 heads of 256 on one: 256 tokens from 0 (256) 38 and 43, 128 at 3000 (512) 55
+// and 56, 64 at 12000 (832) 79 and 70.
+constexpr uint32_t kKv8TileMin = 48;
+constexpr uint32_t kv8_group_wgs(uint32_t hd) { return hd <= 128 ? 1024 : 512; }
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
   const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads, T = kv8_group_tokens(G), w = kv->d.sliding_window;
   auto large = [&](const Kv8Run& r) { return (uint64_t)r.n * G >= kKv8TileMin; };
@@ -473,7 +476,7 @@ void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv
     }
   for (uint32_t i = 0; i < runs.size(); i++) {
     const Kv8Run& r = runs[i];
-    const bool tile = wgs > kKv8GroupWgs && large(r);
+    const bool tile = wgs > kv8_group_wgs(kv->d.head_dim) && large(r);
     for (uint32_t at = 0, m; at < r.n; at += m) {
       const uint32_t pos = r.pos0 + at;
       m = std::min(r.n - at, tile ? kv8_tile_rows(kv->d.head_dim) / G : std::min(T, kKv8Block - pos % kKv8Block));
