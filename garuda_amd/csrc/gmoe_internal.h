@@ -514,16 +514,17 @@ constexpr uint32_t kKv8Split = 512;
 constexpr uint32_t kv8_parts(uint32_t span) { return 1 + (span + kKv8Block - 1 + kKv8Split - 1) / kKv8Split; }
 // Whether the workgroup that finishes last joins a group's parts, or a launch of its own: while
 // a call's workgroups all run at once, and the join is one pass over a few parts, it costs less
-// than a launch (one sequence at 4000: 15.7 us, 18.1 with the launch; 8 at 2047 20.5 and 21.4);
+// than a launch (one sequence at 4000: 15.5 us, 18.4 with the launch; 8 at 2047 20.2 and 22.0);
 // beyond that, writing the parts past the caches and counting them costs every workgroup more
-// (8 sequences at 65000 248 us, 222 with the launch; 32 with 8 heads of 256 on one at 6000 29.7 and 27.9).
+// (8 sequences at 65000 250 us, 220 with the launch; 32 with 8 heads of 256 on one at 6000 29.2 and
+// 27.3; 5 drafts of each of 6 at 6000 36.2 and 33.3).
 constexpr uint32_t kKv8Join = 16, kKv8FusedWgs = 1024;
 constexpr uint32_t kv8_fused(uint32_t items, uint32_t n_kv, uint32_t nparts, uint32_t floats) {  // of a group's context
   return nparts <= kKv8Join && floats <= 4 * 256 && (uint64_t)items * n_kv <= kKv8FusedWgs ? 1 : 0;
 }
 // Rows that a workgroup of the joining launch takes: hd / 4 threads for kKv8Join parts of one, so
-// several where parts are few and workgroups enough (6 sequences' 5 drafts at 3000, a row each
-// 38.2 us, several 34.6; 32 heads of 256 at 6000, 256 rows, 27.0 and 27.7).
+// several where parts are few and workgroups enough (5 drafts of each of 6 sequences, 1536 rows, one a
+// workgroup 38.2 us, several 34.6; 8 heads of 256 of each of 32, 256 rows, 27.0 and 27.7).
 constexpr uint32_t kv8_join_rows(uint32_t hd, uint32_t nparts, uint64_t rows) {
   const uint32_t groups = 256 / (hd / 4), per = (nparts + kKv8Join - 1) / kKv8Join, most = per < groups ? groups / per : 1;
   return rows / 256 < most ? (rows < 512 ? 1 : (uint32_t)(rows / 256)) : most;
@@ -551,7 +552,7 @@ struct Kv8Args {
   float* qr;           // [n][n_heads * hd] rotated queries; null: the call only appends
   float* own;          // [njob][2][n_kv][16][hd]: the jobs' f32 rows, keys rotated,
   float2* own_max;     //   and [njob][n_kv] their largest magnitudes (keys, values)
-  float* part;         // partial sums of the groups' rows (kv8_part_floats): the own block,
+  float* part;         // partial sums of the groups' rows: the own block,
   uint32_t nparts;     //   then as many splits as the longest span has
   uint32_t* done;      // [groups][n_kv] parts that are written; 0 between calls
   uint32_t fused;      // 1: the last workgroup of a group joins its parts (kv8_fused)

@@ -458,13 +458,13 @@ void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
 // at most kv8_tile_rows. A group reads the cache for itself, but a call of few groups has them all on
 // the card at once, where a tile's waves without rows idle; so runs of 48 rows or more go in tiles
 // where as groups they would make more workgroups than the CUs hold (two each, of heads wider than 128
-// one) twice over. 32 heads on 8 of 128, in groups and in tiles: 32 tokens at 3008 (448 workgroups)
-// 31 and 36 us, at 12000 (1600) 53 and 49; 16 tokens of each of 6 sequences at 3008 (1344) 55.5 and
-// 53.7, 32 of each 88 and 58; 12 of each (1008) 46 and 52. 64 tokens at 2000, 8 heads on 2 of 32
-// (160): 19.5 and 27. 8 heads of 256 on one: 256 tokens from 0 (256) 38 and 43, 128 at 3000 (512) 55
-// and 56, 64 at 12000 (832) 79 and 70.
+// one) three times over, of wide heads, whose tiles are smaller, twice. 32 heads on 8 of 128, in groups
+// and in tiles: 32 tokens at 3008 (448 workgroups) 29 and 35 us, at 12000 (1600) 51 and 48; 12 tokens
+// of each of 6 sequences at 3008 (1008) 40 and 50, 16 (1344) 48 and 52, 32 (2688) 73 and 57. 64 tokens
+// at 2000, 8 heads on 2 of 32 (160): 18 and 25. 8 heads of 256 on one: 256 tokens from 0 (256) 39 and
+// 42, 128 at 3000 (512) 56 and 56, 64 at 12000 (832) 79 and 70.
 constexpr uint32_t kKv8TileMin = 48;
-constexpr uint32_t kv8_group_wgs(uint32_t hd) { return hd <= 128 ? 1024 : 512; }
+constexpr uint32_t kv8_group_wgs(uint32_t hd) { return hd <= 128 ? 1536 : 512; }
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
   const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads, T = kv8_group_tokens(G), w = kv->d.sliding_window;
   auto large = [&](const Kv8Run& r) { return (uint64_t)r.n * G >= kKv8TileMin; };
@@ -489,7 +489,7 @@ void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv
 // about one a CU, each split keeping at least two steps of 64 positions. The own blocks get a split
 // of their own where there are CUs for it (of few tiles, one is kept for it): a split of few
 // positions takes as long again for them. 256 tokens at 1280, 32 heads on 8 of 128: 6 splits, the
-// own blocks in the first, 53 us; in a seventh 49.
+// own blocks in the first, 52 us; in a seventh 47.
 constexpr uint32_t kKv8TileWgs = 256;
 uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_t* splits, uint32_t* own) {
   uint32_t span = 1;
