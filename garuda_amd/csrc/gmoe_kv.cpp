@@ -456,18 +456,22 @@ void fill_jobs(const gmoe_kv* kv, uint32_t layer, Plan8& P, Kv8Job* jobs) {
 
 // The runs cut into groups (job: the run's index, for now) of at most 16 rows, or into tiles of
 // at most kv8_tile_rows. A group reads the cache for itself, but a call of few groups has them all on
-// the card at once, where a tile's waves without rows idle; so runs of 48 rows or more go in tiles
+// the card at once, where a tile's waves without rows idle; so runs of enough rows go in tiles
 // where as groups they would make more workgroups than the CUs hold (two each, of heads wider than 128
 // one) three times over, of wide heads, whose tiles are smaller, twice. 32 heads on 8 of 128, in groups
-// and in tiles: 32 tokens at 3008 (448 workgroups) 29 and 35 us, at 12000 (1600) 51 and 48; 12 tokens
-// of each of 6 sequences at 3008 (1008) 40 and 50, 16 (1344) 48 and 52, 32 (2688) 73 and 57. 64 tokens
-// at 2000, 8 heads on 2 of 32 (160): 18 and 25. 8 heads of 256 on one: 256 tokens from 0 (256) 39 and
-// 42, 128 at 3000 (512) 56 and 56, 64 at 12000 (832) 79 and 70.
-constexpr uint32_t kKv8TileMin = 48;
+// and in tiles: 32 tokens at 3008 (448 workgroups) 29 and 35 us, at 12000 (1600) 51 and 48; 16 tokens
+// of each of 6 sequences at 3008 (1344) 48 and 52, 32 (2688) 73 and 57. 64 tokens at 2000, 8 heads on 2
+// of 32 (160): 18 and 25. 8 heads of 256 on one: 256 tokens from 0 (256) 39 and 42, 128 at 3000 (512)
+// 56 and 56, 64 at 12000 (832) 79 and 70.
+// Enough rows, of a run alone in its tile: what a step of a tile costs beside its products does not
+// shrink with the rows, nor with the heads. 30 sequences at 3008: 48 and 64 rows of 128 131 and 160, 167
+// and 163; 80 and 96 of 64 216 and 244, 259 and 255; 63 and 96 of 80 87 and 95, 129 and 97; 128 of 32
+// 41 and 46; 56 of 256 76 and 62.
+constexpr uint32_t kv8_tile_min(uint32_t hd) { return 32 + 4096 / kv8_width(hd); }
 constexpr uint32_t kv8_group_wgs(uint32_t hd) { return hd <= 128 ? 1536 : 512; }
 void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv8Run>& groups, std::vector<Kv8Run>& tiles) {
   const uint32_t G = kv->d.n_heads / kv->d.n_kv_heads, T = kv8_group_tokens(G), w = kv->d.sliding_window;
-  auto large = [&](const Kv8Run& r) { return (uint64_t)r.n * G >= kKv8TileMin; };
+  auto large = [&](const Kv8Run& r) { return (uint64_t)r.n * G >= kv8_tile_min(kv->d.head_dim); };
   uint64_t wgs = 0;
   for (const Kv8Run& r : runs)
     if (large(r)) {

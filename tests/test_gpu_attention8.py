@@ -127,9 +127,10 @@ def test_steps_and_prompts_of_every_head_layout(dev, nh, nkv, hd):
 
 
 def in_tiles(nh, nkv, hd, spans, window=0):
-    """Whether a call of runs (start, end) of 48 rows or more goes in tiles: as groups of 16 rows and splits of
+    """Whether a call of runs (start, end) of 160 rows or more goes in tiles: as groups of 16 rows and splits of
     their spans it would make more than 1536 workgroups, of heads wider than 128 more than 512."""
     g = nh // nkv
+    assert all((e - s) * g >= 160 for s, e in spans)
     first = [max(0, e - window) // BLOCK * BLOCK if window else 0 for _, e in spans]
     wgs = sum(-(-(e - s) // (16 // g)) * (1 + -(-((e - 1) // BLOCK * BLOCK - f) // 512)) * nkv for (s, e), f in zip(spans, first))
     return wgs > (1536 if hd <= 128 else 512)
