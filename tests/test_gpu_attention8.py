@@ -503,6 +503,21 @@ def test_far_positions_turn_exactly(dev):
         assert np.array_equal(got, held[:, 0])
 
 
+def test_more_parts_than_a_pass_joins(dev):
+    # heads of 256: four threads' groups of 16 parts of 512 positions are 32768 positions
+    nh, nkv, hd, n = 2, 1, 256, 40005
+    rng = np.random.default_rng(18)
+    with KvCache(dev, 1, nh, nkv, hd, block_size=64, max_positions=n + 40, max_seqs=2, bits=8) as kv:
+        o = Kv8Oracle(1, nh, nkv, hd, max_positions=n + 40)
+        a, b = kv.open_seq(), kv.open_seq()
+        for s, m in ((a, n), (b, 700)):
+            k, v = draw(rng, m, nh, nkv, hd)[1:]
+            kv.append(0, [s] * m, k, v)
+            o.append(0, [s] * m, k, v)
+        run(kv, o, 0, [a, b], draw(rng, 2, nh, nkv, hd), "many parts, a step")
+        run(kv, o, 0, [b, a, a, a], draw(rng, 4, nh, nkv, hd), "many parts, drafts")
+
+
 def test_streams_and_a_run_of_them_together(dev):
     """A prompt shared by three sequences, appended once each without attention; decode steps on a
     stream of the caller's; drafted tokens checked in one call and half of them taken back; the
