@@ -409,7 +409,10 @@ __device__ float uniform_mean(const Kv8Pool& p, uint32_t table, uint32_t h, uint
     for (uint32_t r = 0; r < kKv8Block; r++) n += b * kKv8Block + r >= start ? (int)c[r] - 128 : 0;
     sum += (double)n * (double)p.scales[2 * u + 1];
   }
-  for (uint32_t r = start > own ? start - own : 0; r <= pos - own; r++) sum += (double)(shared ? __hip_atomic_load(vo + r * vstride + d, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : vo[r * vstride + d]);
+  for (uint32_t r = start > own ? start - own : 0; r <= pos - own; r++) {
+    const float* v = vo + r * vstride + d;
+    sum += (double)(shared ? __hip_atomic_load(v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : *v);
+  }
   return (float)(sum / (double)(pos + 1 - start));
 }
 
@@ -1118,9 +1121,9 @@ __device__ __forceinline__ void rows_again(const Kv8Args& a, const Kv8Run& run, 
 // 16 scores of 32 positions are 8 consecutive ones of each of two blocks, its own half of
 // the second product's B operand; O^T = V^T P^T.
 //
-// Split 0 takes the rows' own blocks after its positions, or by itself, 32 positions at a time: f32 rows, scaled by a power of
-// two for each block, as two fp16 each, three of the four products of two such sums (the
-// fourth is 2^-22 of the first). A row that meets a score that is NaN or +inf, or whose own block
+// Split 0 takes the rows' own blocks after its positions, or by itself, 32 positions at a time: f32
+// rows, scaled by a power of two for each block, as two fp16 each, three of the four products of
+// two such sums (the fourth is 2^-22 of the first). A row that meets a score that is NaN or +inf, or whose own block
 // has a value that is not finite, is marked and summed again by itself in f32 (row_again).
 //
 // The sums of 32 rows of 256 are half the registers that a SIMD has for one wave: it runs alone, its

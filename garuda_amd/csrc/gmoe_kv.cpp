@@ -912,7 +912,8 @@ void kv_commit_step(gmoe_kv* kv, const uint32_t* seqs, uint32_t n, AttnEntry* en
   for (uint32_t l = 0; l < kv->d.n_layers; l++) commit(kv, l, seqs, n, ents + (size_t)l * stride);
 }
 
-static size_t open_bytes(const gmoe_kv* kv) { return (size_t)kv->d.n_layers * 2 * kKv8Block * kv->kvd * 4; }  // a sequence's open rows, every layer's
+// A sequence's open rows, every layer's.
+static size_t open_bytes(const gmoe_kv* kv) { return (size_t)kv->d.n_layers * 2 * kKv8Block * kv->kvd * 4; }
 
 // The step's sequences as they stand (every layer's length and page count), and their
 // return to it: pages taken since go back to the free list, lengths go back. A step that
@@ -1006,7 +1007,8 @@ gmoe_status kv_attend_dev(gmoe_kv* kv, uint32_t n, const AttnEntry* d_ent, uint3
     a.nparts = kv8_parts(nchunk * kAttnChunk);
     a.items = n * a.nparts;
     a.fused = kv8_fused(a.items, kv->d.n_kv_heads, a.nparts, kv->d.n_heads / kv->d.n_kv_heads * kv->d.head_dim);
-    if (step_bytes(kv, n, nchunk) > kv->scratch_bytes || (size_t)n * kv->d.n_kv_heads > kv->n_done) return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
+    if (step_bytes(kv, n, nchunk) > kv->scratch_bytes || (size_t)n * kv->d.n_kv_heads > kv->n_done)
+      return kfail(GMOE_ERR_INFERENCE, "attention scratch not reserved");
     KV_TRY(launch_kv8_step(a, Kv8Inline{}, st));
     return GMOE_OK;
   }
@@ -1043,8 +1045,9 @@ static gmoe_status kv_create(gmoe_ctx* ctx, const gmoe_kv_desc* desc, bool q8, g
     return kfail(GMOE_ERR_MODEL, "block_size %u must be a multiple of %u, the positions that share a scale", D.block_size,
                  kKv8Block);
   // pages have numbers of 32 bits, and 2^48 bytes are more than any card's
-  if (D.max_pages > 0xffffffffull || (double)D.max_pages * D.block_size * D.n_kv_heads * D.head_dim > 0x1p48 ||
-      (double)D.max_seqs * D.n_layers * std::max((double)D.max_positions / D.block_size, (double)D.n_kv_heads * D.head_dim) > 0x1p48)
+  const double kvd = (double)D.n_kv_heads * D.head_dim;
+  if (D.max_pages > 0xffffffffull || (double)D.max_pages * D.block_size * kvd > 0x1p48 ||
+      (double)D.max_seqs * D.n_layers * std::max((double)D.max_positions / D.block_size, kvd) > 0x1p48)
     return kfail(GMOE_ERR_CONFIG, "a KV cache of %llu pages and %u sequences is too large",
                  (unsigned long long)D.max_pages, D.max_seqs);
   std::unique_ptr<gmoe_kv> kv(new gmoe_kv);
