@@ -489,11 +489,14 @@ void cut_runs(const gmoe_kv* kv, const std::vector<Kv8Run>& runs, std::vector<Kv
   }
 }
 
-// Positions of a tile's split: the tiles' keys are split over workgroups until the call has
-// about one a CU, each split keeping at least two steps of 64 positions. The own blocks get a split
-// of their own where there are CUs for it (of few tiles, one is kept for it): a split of few
-// positions takes as long again for them. 256 tokens at 1280, 32 heads on 8 of 128: 6 splits, the
-// own blocks in the first, 52 us; in a seventh 47.
+// Positions of a tile's split, at least two steps of 64. Where a CU each leaves room for four splits
+// or more, as many as there are CUs, but for one kept for the own blocks, which then have a split of their
+// own: a split of few positions takes as long again for them (256 tokens at 1280, 32 heads on 8 of
+// 128: 6 splits, the own blocks in the first, 52 us; in a seventh 47). Otherwise the number under which
+// the call would end first, counted in steps: a workgroup's start and end take two, the own blocks
+// one and a half for each 32 positions, the sums of 32 workgroups written and joined one. (Rounded up
+// to a workgroup a CU at least, a second round is mostly empty: 600 tokens at 4000 in 4 splits 163 us, in 3
+// 125; 4 times 300 at 3000 in 2 230, in 1 196 to 209.)
 constexpr uint32_t kKv8TileWgs = 256;
 uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_t* splits, uint32_t* own) {
   uint32_t span = 1;
@@ -502,8 +505,30 @@ uint32_t tile_split(const gmoe_kv* kv, const std::vector<Kv8Run>& tiles, uint32_
     span = std::max(span, (t.pos0 + t.n - 1) / kKv8Block * kKv8Block - std::min(t.pos0, from) / kKv8Block * kKv8Block);
   }
   const uint32_t steps = (span + 63) / 64, wgs = (uint32_t)tiles.size() * kv->d.n_kv_heads;
-  const uint32_t most = kKv8TileWgs / wgs >= 4 ? kKv8TileWgs / wgs - 1 : (kKv8TileWgs + wgs - 1) / wgs;
-  const uint32_t ns = std::max(1u, std::min(most, steps / 2));
+  uint32_t ns = kKv8TileWgs / wgs - 1;
+  if (kKv8TileWgs / wgs < 4) {
+    const uint32_t own_steps = 3 * (kv8_tile_rows(kv->d.head_dim) / (kv->d.n_heads / kv->d.n_kv_heads) + 16) / 64;
+    auto cost = [&](uint32_t n) -> uint64_t {
+      const uint64_t each = (steps + n - 1) / n + 2, first = each + own_steps, left = (uint64_t)wgs * (n - 1);
+      // the first splits start first: then `late` CUs are free at t1, the others at t0
+      const uint64_t late = wgs % kKv8TileWgs, t0 = wgs / kKv8TileWgs * first, t1 = late ? t0 + first : t0;
+      auto done = [&](uint64_t t) {  // of the others by then
+        return (kKv8TileWgs - late) * ((t - t0) / each) + (t > t1 ? late * ((t - t1) / each) : 0);
+      };
+      uint64_t end = t1;
+      if (left) {
+        uint64_t a = t0, b = t1;
+        while (done(a) < left) a += each;
+        while (done(b) < left) b += each;
+        end = std::max(t1, std::min(a, b));
+      }
+      return end + (n > 1 ? (uint64_t)wgs * n / 32 : 0);
+    };
+    ns = 1;
+    for (uint32_t n = 2; n <= 8; n++)
+      if (cost(n) < cost(ns)) ns = n;
+  }
+  ns = std::max(1u, std::min(ns, steps / 2));
   const uint32_t keys = (steps + ns - 1) / ns * 64;
   *splits = (span + keys - 1) / keys;
   *own = *splits > 1 && wgs * (*splits + 1) <= kKv8TileWgs ? 1 : 0;
